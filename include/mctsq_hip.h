@@ -244,6 +244,48 @@ int mctsq_clip_adam_polyak_ex(float* d_params, const float* d_grad, float* d_m, 
 /* Polyak / hard sync alone: target <- tau*policy + (1-tau)*target (dqn_per.py:515-516). */
 int mctsq_polyak(const float* d_params, float* d_target, int64_t n, double tau, void* stream);
 
+/* ---- what a policy learns from.  One row of logits per token, V = vocab (or actions) wide:
+ *   logp_i = z_i[a_i] - log sum_j exp z_i[j]
+ * Logits: dtype 0 fp32, 1 bf16, 2 fp16; `rows` rows in groups of `inner` (rows is a multiple of it), row i starting at
+ * element (i / inner) * stride_outer + (i % inner) * stride_inner, its elements contiguous; any alignment that the type
+ * has, offsets of any size.  d_act: rows integers of act_bytes (4 or 8) bytes.  d_weight fp32 [rows] or NULL (all 1):
+ * a row of weight 0 is padding - its logits and action are never read, its outputs are exactly 0.  An action outside
+ * [0, V) on a row that has weight makes that row's outputs, and the loss, NaN.  Statistics are joined in fp64, in a fixed
+ * order: the same inputs give the same bits.  No reference counterpart (the reference learns from TD errors only).
+ *
+ * mctsq_token_logprobs: d_logp fp32 [rows].
+ *
+ * mctsq_policy_loss: with r = exp(logp - old), k = exp(ref - logp) - (ref - logp) - 1,
+ *   loss = loss_scale * sum_i w_i (-min(r_i A_i, clip(r_i, 1 - clip_low, 1 + clip_high) A_i) + kl_coef k_i)
+ * d_old_logp fp32 [rows] or NULL (on-policy: r = 1); d_ref_logp fp32 [rows] or NULL (no KL term); d_adv: row i uses
+ * d_adv[i / adv_div] (adv_div = 1: one per row; = inner: one per sequence).  Outputs: d_loss [1], d_logp [rows],
+ * d_kl [rows] (k_i; 0 without a reference), d_dlogits or NULL: the gradient of the loss in the logits' type with its own
+ * strides; it may be the logits themselves (same pointer and strides), else must not overlap them.  Where the unclipped
+ * product equals the clipped one the gradient is the unclipped one's.
+ *
+ * mctsq_preference_loss: 2 * pairs sequences of `tokens` rows, the preferred ones first; S_q = sum_t w_qt logp_qt,
+ *   h_p = beta ((S_p - R_p) - (S_{p+pairs} - R_{p+pairs})),
+ *   loss = loss_scale * sum_p u_p (-(1 - e) log sigmoid(h_p) - e log sigmoid(-h_p)),   e = label_smoothing in [0, 0.5]
+ * d_ref_logp fp32 [2 * pairs]: the reference policy's sums R; d_pair_weight fp32 [pairs] or NULL: u (0: a padding pair, its
+ * rows are not read and its outputs are 0).  Outputs: d_loss [1], d_seq_logp [2 * pairs], d_margin [pairs] (h),
+ * d_dlogits as above (the logits may be overwritten by it). */
+int mctsq_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t inner, int64_t stride_outer,
+                         int64_t stride_inner, int64_t vocab, const void* d_act, int act_bytes, const float* d_weight,
+                         float* d_logp, void* stream);
+int64_t mctsq_policy_loss_workspace_bytes(int64_t rows);
+int mctsq_policy_loss(const void* d_logits, int dtype, int64_t rows, int64_t inner, int64_t stride_outer,
+                      int64_t stride_inner, int64_t vocab, const void* d_act, int act_bytes, const float* d_old_logp,
+                      const float* d_ref_logp, const float* d_adv, int64_t adv_div, const float* d_weight,
+                      double clip_low, double clip_high, double kl_coef, double loss_scale, float* d_loss, float* d_logp,
+                      float* d_kl, void* d_dlogits, int64_t dstride_outer, int64_t dstride_inner, void* d_ws,
+                      int64_t ws_bytes, void* stream);
+int64_t mctsq_preference_loss_workspace_bytes(int64_t pairs, int64_t tokens);
+int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pairs, int64_t tokens, int64_t stride_outer,
+                          int64_t stride_inner, int64_t vocab, const void* d_act, int act_bytes, const float* d_ref_logp,
+                          const float* d_weight, const float* d_pair_weight, double beta, double label_smoothing,
+                          double loss_scale, float* d_loss, float* d_seq_logp, float* d_margin, void* d_dlogits,
+                          int64_t dstride_outer, int64_t dstride_inner, void* d_ws, int64_t ws_bytes, void* stream);
+
 /* ---- prioritized replay: PrioritizedReplayBuffer (dqn_per.py:238-321) as a device-resident
  * ring + 64-ary integer sum-tree.  Logical index 0 is the OLDEST entry (deque(maxlen)).
  * Priorities are fp64; probability mass m = rint(min(prio^alpha, 256) * 2^shift) as uint64 (deterministic

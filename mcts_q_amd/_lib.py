@@ -73,6 +73,13 @@ SIGNATURES = {
     "mctsq_clip_adam_polyak": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f64, _f64, _f64, _f64, _f64,
                                       _f64, _vp, _vp, _i64, _vp]),
     "mctsq_polyak": (_i32, [_vp, _vp, _i64, _f64, _vp]),
+    "mctsq_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp]),
+    "mctsq_policy_loss_workspace_bytes": (_i64, [_i64]),
+    "mctsq_policy_loss": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _vp]
+                          + [_f64] * 4 + [_vp] * 4 + [_i64, _i64, _vp, _i64, _vp]),
+    "mctsq_preference_loss_workspace_bytes": (_i64, [_i64, _i64]),
+    "mctsq_preference_loss": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp] + [_f64] * 3
+                              + [_vp] * 4 + [_i64, _i64, _vp, _i64, _vp]),
     "mctsq_per_tree_words": (_i64, [_i64]),
     "mctsq_per_mass_shift": (_i32, [_i64]),
     "mctsq_per_workspace_bytes": (_i64, [_i64, _i64]),
