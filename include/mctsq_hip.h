@@ -286,6 +286,33 @@ int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pairs, int64_
                           double loss_scale, float* d_loss, float* d_seq_logp, float* d_margin, void* d_dlogits,
                           int64_t dstride_outer, int64_t dstride_inner, void* d_ws, int64_t ws_bytes, void* stream);
 
+/* ---- orthogonalised updates.  For every matrix, with u the matrix given (orthogonalize) or its momentum-averaged gradient:
+ *   X = u / (|u|_F + eps);  five times  A = X X^T, X <- 3.4445 X + (-4.7750 A + 2.0315 A^2) X
+ * (on the transpose where rows > cols), which takes the singular values that are not negligible to about 1.
+ * mctsq_orthogonalize: d_out <- X, in the matrices' type (dtype 0 fp32, 1 bf16); d_out may be d_x.
+ * mctsq_muon_step:  m <- momentum m + g;  u = g + momentum m (nesterov) or m;
+ *                   p <- p (1 - lr weight_decay) - lr f X,  f = 1 (NONE), sqrt(max(1, rows / cols)) (SPECTRAL),
+ *                   0.2 sqrt(max(rows, cols)) (RMS: the update's root mean square matches an Adam step's)
+ * p = d_out, m = d_momentum (contiguous [rows][cols]) in fp32, g = d_x in grad_dtype.  fp32 matrices and the step are
+ * evaluated to fp32 accuracy, bf16 matrices to bf16 accuracy (operands of the products in 11 bits, sums in fp32).
+ * ld*: elements between rows.  Sides up to 65536, any number of matrices of any mixture of shapes; the same inputs give the
+ * same bits.  A matrix that holds an infinity or NaN becomes NaN.  `mats` is read by the host during the call only; matrices
+ * must not overlap.  d_ws: the matching *_workspace_bytes() of the same list, 256-byte aligned; its contents are scratch.
+ * No reference counterpart (the reference updates by Adam). */
+enum { MCTSQ_MUON_NONE = 0, MCTSQ_MUON_SPECTRAL = 1, MCTSQ_MUON_RMS = 2 };
+typedef struct {
+    int64_t rows, cols;
+    const void* d_x; int64_t ldx;
+    float* d_momentum;
+    void* d_out; int64_t ldo;
+} mctsq_muon_matrix;
+int64_t mctsq_orthogonalize_workspace_bytes(const mctsq_muon_matrix* mats, int64_t count, int dtype);
+int mctsq_orthogonalize(const mctsq_muon_matrix* mats, int64_t count, int dtype, double eps, void* d_ws, int64_t ws_bytes,
+                        void* stream);
+int64_t mctsq_muon_workspace_bytes(const mctsq_muon_matrix* mats, int64_t count);
+int mctsq_muon_step(const mctsq_muon_matrix* mats, int64_t count, int grad_dtype, double lr, double momentum, int nesterov,
+                    double weight_decay, double eps, int adjust, void* d_ws, int64_t ws_bytes, void* stream);
+
 /* ---- prioritized replay: PrioritizedReplayBuffer (dqn_per.py:238-321) as a device-resident
  * ring + 64-ary integer sum-tree.  Logical index 0 is the OLDEST entry (deque(maxlen)).
  * Priorities are fp64; probability mass m = rint(min(prio^alpha, 256) * 2^shift) as uint64 (deterministic

@@ -40,6 +40,12 @@ class StepArgs(C.Structure):
                 + [(n, _i64) for n in ("world", "rank", "bcap")]
                 + [(n, _vp) for n in ("d_shard_mass", "d_shard_size", "d_count", "d_draw", "d_exchange")])
 
+class MuonMatrix(C.Structure):
+    """mctsq_muon_matrix (include/mctsq_hip.h)."""
+    _fields_ = [("rows", _i64), ("cols", _i64), ("d_x", _vp), ("ldx", _i64), ("d_momentum", _vp), ("d_out", _vp),
+                ("ldo", _i64)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/mctsq_hip.h
 SIGNATURES = {
     "mctsq_abi_version": (_i32, []),
@@ -80,6 +86,10 @@ SIGNATURES = {
     "mctsq_preference_loss_workspace_bytes": (_i64, [_i64, _i64]),
     "mctsq_preference_loss": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp] + [_f64] * 3
                               + [_vp] * 4 + [_i64, _i64, _vp, _i64, _vp]),
+    "mctsq_orthogonalize_workspace_bytes": (_i64, [_vp, _i64, _i32]),
+    "mctsq_orthogonalize": (_i32, [_vp, _i64, _i32, _f64, _vp, _i64, _vp]),
+    "mctsq_muon_workspace_bytes": (_i64, [_vp, _i64]),
+    "mctsq_muon_step": (_i32, [_vp, _i64, _i32, _f64, _f64, _i32, _f64, _f64, _i32, _vp, _i64, _vp]),
     "mctsq_per_tree_words": (_i64, [_i64]),
     "mctsq_per_mass_shift": (_i32, [_i64]),
     "mctsq_per_workspace_bytes": (_i64, [_i64, _i64]),
@@ -157,3 +167,23 @@ def ptr(t):
         return t.data_ptr()
     except AttributeError:
         return t.ctypes.data
+
+
+class on_device:
+    """`with on_device(t.device):` launches go to that device whichever is current (torch.cuda.device costs ten times
+    this where nothing has to change, and these calls are host-bound when they are small)."""
+    __slots__ = ("device", "prev")
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        import torch
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.device.index:
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *exc):
+        import torch
+        if self.prev != self.device.index:
+            torch.cuda.set_device(self.prev)

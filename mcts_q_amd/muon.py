@@ -1,0 +1,141 @@
+"""Orthogonalised updates on device tensors through libmctsq_hip.so: the quintic Newton-Schulz iteration on matrices
+(`orthogonalize`) and the optimizer whose step it is (`DeviceMuon`).
+
+The iteration replaces a matrix by roughly the nearest semi-orthogonal one: X = x / |x|_F, then five times
+X <- 3.4445 X + (-4.7750 A + 2.0315 A^2) X with A = X X^T.  fp32 matrices are evaluated to fp32 accuracy, bf16 matrices to
+bf16 accuracy.  Everything is enqueued on the current stream of the tensors' device; nothing synchronises."""
+from __future__ import annotations
+
+import torch
+
+from ._lib import MctsqError, MuonMatrix, lib, on_device, ptr, stream_ptr
+
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
+_ADJUST = {"none": 0, "spectral": 1, "rms": 2}
+_ALIGN = 256
+
+
+def _aligned(nbytes, device):
+    buf = torch.empty(nbytes + _ALIGN, dtype=torch.uint8, device=device)
+    off = -buf.data_ptr() % _ALIGN
+    return buf[off:off + nbytes]
+
+
+def _is_matrix(t):
+    """[rows, cols] or [count, rows, cols] with at least one element and contiguous rows."""
+    return t.dim() in (2, 3) and t.numel() > 0 and (t.shape[-1] == 1 or t.stride(-1) == 1) \
+        and (t.shape[-2] == 1 or t.stride(-2) >= t.shape[-1])
+
+
+def _ld(t):
+    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+
+
+def _slices(t):
+    """(data pointer) of every matrix of a stack."""
+    if t.dim() == 2:
+        return [t.data_ptr()]
+    step = t.stride(0) * t.element_size()
+    return [t.data_ptr() + i * step for i in range(t.shape[0])]
+
+
+def orthogonalize(x, eps=1e-7, out=None):
+    """The iteration on `x` [rows, cols] or each matrix of [count, rows, cols], fp32 or bf16, rows contiguous.  Returns a
+    tensor of the same shape and type (`out` if given; `out` may be `x`)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise MctsqError("orthogonalize needs a tensor on the GPU: the HIP path has no CPU fallback")
+    if x.dtype not in _DTYPE:
+        raise ValueError(f"x: expected fp32 or bf16, got {x.dtype}")
+    if not _is_matrix(x):
+        raise ValueError(f"x: expected [rows, cols] or [count, rows, cols] with contiguous rows, got {tuple(x.shape)} "
+                         f"with strides {x.stride()}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not _is_matrix(out) \
+            or (out.dim() == 3 and out.shape[0] > 1 and out.stride(0) < (out.shape[1] - 1) * _ld(out) + out.shape[2]):
+        raise ValueError(f"out: expected {tuple(x.shape)} {x.dtype} on {x.device} with contiguous rows that do not overlap")
+    r, c = x.shape[-2:]
+    src, dst = _slices(x), _slices(out)
+    lx, lo = _ld(x), _ld(out)
+    mats = (MuonMatrix * len(src))(*[MuonMatrix(r, c, s, lx, None, d, lo) for s, d in zip(src, dst)])
+    dt = _DTYPE[x.dtype]
+    with on_device(x.device):
+        need = lib.check(lib.mctsq_orthogonalize_workspace_bytes(mats, len(src), dt))
+        ws = _aligned(need, x.device)
+        lib.check(lib.mctsq_orthogonalize(mats, len(src), dt, eps, ptr(ws), need, stream_ptr(x.device)))
+    return out
+
+
+class DeviceMuon:
+    """Muon over a list of fp32 weight matrices, updated in place.
+
+        m <- momentum m + g;  u = g + momentum m (nesterov) or m
+        p <- p (1 - lr weight_decay) - lr f orthogonalize(u)
+
+    f by `adjust`: "spectral" sqrt(max(1, rows / cols)), "rms" 0.2 sqrt(max(rows, cols)), "none" 1.  A parameter is
+    [rows, cols] or a stack [count, rows, cols] of matrices, rows contiguous.  Gradients are fp32 or bf16, all of one type.
+    `momentum_buffers` (fp32, contiguous, one per parameter) is the state; the workspace is kept, so steps of one instance
+    belong on one stream at a time (two graphs captured from one instance must not run at once)."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, eps=1e-7, adjust="spectral",
+                 momentum_buffers=None):
+        params = list(params)
+        if not params:
+            raise ValueError("params: empty")
+        for i, p in enumerate(params):
+            if not isinstance(p, torch.Tensor) or not p.is_cuda:
+                raise MctsqError("DeviceMuon needs parameters on the GPU: the HIP path has no CPU fallback")
+            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != params[0].device \
+                    or (p.dim() == 3 and p.shape[0] > 1 and p.stride(0) < (p.shape[1] - 1) * _ld(p) + p.shape[2]):
+                raise ValueError(f"params[{i}]: expected fp32 [rows, cols] or [count, rows, cols] with contiguous rows on "
+                                 f"{params[0].device}, got {tuple(p.shape)} {p.dtype} with strides {p.stride()} on {p.device}")
+        if adjust not in _ADJUST:
+            raise ValueError(f"adjust: expected one of {sorted(_ADJUST)}, got {adjust!r}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"momentum must lie in [0, 1), got {momentum}")
+        self.params, self.device = params, params[0].device
+        self.lr, self.momentum, self.nesterov = float(lr), float(momentum), bool(nesterov)
+        self.weight_decay, self.eps, self.adjust = float(weight_decay), float(eps), adjust
+        if momentum_buffers is None:
+            momentum_buffers = [torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in params]
+        for i, (p, m) in enumerate(zip(params, momentum_buffers, strict=True)):
+            if m.shape != p.shape or m.dtype != torch.float32 or m.device != p.device or not m.is_contiguous():
+                raise ValueError(f"momentum_buffers[{i}]: expected contiguous fp32 {tuple(p.shape)} on {p.device}")
+        self.momentum_buffers = list(momentum_buffers)
+        mats, self._spans = [], []
+        for p, m in zip(params, self.momentum_buffers):
+            ps, ms = _slices(p), _slices(m)
+            self._spans.append((len(mats), len(ps)))
+            mats += [MuonMatrix(p.shape[-2], p.shape[-1], None, 0, b, a, _ld(p)) for a, b in zip(ps, ms)]
+        self._mats = (MuonMatrix * len(mats))(*mats)
+        with on_device(self.device):
+            self._ws_bytes = lib.check(lib.mctsq_muon_workspace_bytes(self._mats, len(mats)))
+            self._ws = _aligned(self._ws_bytes, self.device)
+
+    def step(self, grads, lr=None):
+        """One update from `grads` (a sequence in the order of the parameters)."""
+        if len(grads) != len(self.params):
+            raise ValueError(f"grads: expected {len(self.params)} tensors, got {len(grads)}")
+        dt = grads[0].dtype
+        if dt not in _DTYPE:
+            raise ValueError(f"grads: expected fp32 or bf16, got {dt}")
+        for i, (g, p, (at, k)) in enumerate(zip(grads, self.params, self._spans)):
+            if g.shape != p.shape or g.dtype != dt or g.device != self.device or not _is_matrix(g):
+                raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {dt} on {self.device} with contiguous rows, got "
+                                 f"{tuple(g.shape)} {g.dtype} with strides {g.stride()} on {g.device}")
+            ld = _ld(g)
+            for j, q in enumerate(_slices(g)):
+                self._mats[at + j].d_x, self._mats[at + j].ldx = q, ld
+        with on_device(self.device):
+            lib.check(lib.mctsq_muon_step(self._mats, len(self._mats), _DTYPE[dt], self.lr if lr is None else float(lr),
+                                          self.momentum, int(self.nesterov), self.weight_decay, self.eps,
+                                          _ADJUST[self.adjust], ptr(self._ws), self._ws_bytes, stream_ptr(self.device)))
+
+    def state_dict(self):
+        return {"momentum_buffers": [m.clone() for m in self.momentum_buffers]}
+
+    def load_state_dict(self, sd):
+        for m, s in zip(self.momentum_buffers, sd["momentum_buffers"], strict=True):
+            if tuple(s.shape) != tuple(m.shape):
+                raise ValueError(f"momentum buffer: expected {tuple(m.shape)}, got {tuple(s.shape)}")
+            m.copy_(s)

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import MctsqError, lib, ptr, stream_ptr
+from ._lib import MctsqError, lib, on_device, ptr, stream_ptr
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -74,29 +74,13 @@ def _out_strides(out):
     return (0, out.stride(0)) if out.dim() == 2 else (out.stride(0), out.stride(1))
 
 
-class _On:
-    """Launches go to the tensors' device whichever is current."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.device.index:
-            torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.prev != self.device.index:
-            torch.cuda.set_device(self.prev)
-
-
 def token_logprobs(logits, actions, weight=None):
     """log pi(action) of every row, fp32 in the leading shape (0 where weight is 0)."""
     n, inner, so, si, V, lead = _rows(logits, actions)
     dev = logits.device
     _vec("weight", weight, lead, dev)
     logp = torch.empty(lead, dtype=torch.float32, device=dev)
-    with _On(dev):
+    with on_device(dev):
         lib.check(lib.mctsq_token_logprobs(ptr(logits), _DTYPE[logits.dtype], n, inner, so, si, V, ptr(actions),
                                            actions.element_size(), ptr(weight), ptr(logp), stream_ptr(dev)))
     return logp
@@ -126,7 +110,7 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, weight=Non
         raise ValueError("out is given but grad is False")
     d = _grad_out(logits, out) if grad else None
     dso, dsi = _out_strides(d) if grad else (0, 0)
-    with _On(dev):
+    with on_device(dev):
         need = lib.check(lib.mctsq_policy_loss_workspace_bytes(n))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         loss = torch.empty(1, dtype=torch.float32, device=dev)
@@ -164,7 +148,7 @@ def preference_loss(logits, actions, ref_logp, weight=None, beta=0.1, label_smoo
         loss_scale = 1.0 / max(P, 1)
     d = _grad_out(logits, out) if grad else None
     dso, dsi = _out_strides(d) if grad else (0, 0)
-    with _On(dev):
+    with on_device(dev):
         need = lib.check(lib.mctsq_preference_loss_workspace_bytes(P, T))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         loss = torch.empty(1, dtype=torch.float32, device=dev)
