@@ -4,15 +4,15 @@
 //   logp_i = z_i[a_i] - lse_i,   lse_i = log sum_j exp z_i[j],   d logp_i / d z_i[j] = [j = a_i] - p_i[j]
 //
 // so every loss here is a coefficient c_i = d loss / d logp_i per row and the gradient row c_i (one_hot(a_i) - p_i).
-// The bound is HBM: each logit read once, each gradient element written once.  One workgroup owns a row at a time:
-//   - the row is loaded ONCE into registers as the 16-byte vectors it arrives in (row_reg_kernel), every thread reduces
-//     its own elements to (max, sum of exponentials), the pairs are joined over the workgroup with one barrier, thread 0
-//     turns them into the coefficient, and the gradient is formed from the same registers;
-//   - rows longer than the registers hold are read twice (row_stream_kernel), the second time from the caches;
-//   - rows of at most 256 elements go to groups of 4 or 16 lanes (row_lane_kernel), many rows to a workgroup.
-// Statistics: exponentials and per-thread sums in fp32 (at most 128 terms), everything joined across threads, the
-// logarithm, ratio, KL term and loss in fp64: the clip decides on a ratio that two evaluations must agree on.
-// Rows of weight 0 are padding: their logits, action, and statistics are not read, their outputs are exactly 0.
+// The bound is HBM: each logit read once, each gradient element written once; the exponentials are the next one.
+//   - rows of more than 256 elements: RW waves own a row at a time and take it in 16-byte vectors, U of them in flight per
+//     lane, every lane with a running (max, sum of exponentials); the pairs are joined over the waves with one barrier, one
+//     thread turns them into the coefficient.  Where U vectors a lane hold the whole row (HOLD), the exponentials stay in
+//     registers and the gradient is one product per element; longer rows are read a second time, now from the caches.
+//   - rows of at most 256 elements go to groups of 4 or 16 lanes and stay in registers, many rows to a workgroup.
+// Statistics: exponentials and the sums of one lane in fp32 (at most 32 terms between two rescalings), everything joined
+// across lanes, the logarithm, ratio, KL term and loss in fp64: the clip decides on a ratio that two evaluations must agree
+// on.  Rows of weight 0 are padding: their logits, action, and statistics are not read, their outputs are exactly 0.
 // An action outside [0, V) on a row that has weight makes that row's outputs and the loss NaN; nothing is read for it.
 // Sums are joined in a fixed order: the same inputs give the same bits.
 #include <float.h>
@@ -29,6 +29,7 @@ struct RowArgs {
     const char* z; int64_t z_so, z_si;        // logits and their strides (elements): row i = (i / inner, i % inner)
     char* dz; int64_t d_so, d_si;             // gradient (may be the logits themselves), NULL: none
     int64_t rows, inner, V;
+    int one_group;                            // inner == all rows: nothing to divide
     const void* act; int act64;
     const float* w;                           // row weights, NULL: 1
     const float* pair_w; int64_t pairs;       // pair weights of the preference loss (row / inner = pair or pairs + pair)
@@ -36,7 +37,7 @@ struct RowArgs {
     const float* old_logp; const float* ref_logp; const float* adv; int64_t adv_div;
     double clip_lo, clip_hi, kl_coef, scale;
     float* logp; float* kl;
-    double* loss_part;                        // one per workgroup
+    double* loss_part; float* loss;           // one part per workgroup, or the loss itself from a launch of one
     // preference: statistics of pass 1 (read by pass 2), coefficient per sequence
     double* logp64; float* stat_m; float* stat_inv; const float* seq_coef;
 };
@@ -115,16 +116,20 @@ struct RowView {
         if (e0 >= 0 && e0 + VE <= V) return *reinterpret_cast<const u32x4*>(base + e0 * (int64_t)sizeof(T));
         u32x4 u;
         u[0] = u[1] = u[2] = u[3] = Elem<T>::NEG_INF;
+        u32x4 c;                                            // element by element, all loads at once
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
             const int64_t e = e0 + j;
-            if (e >= 0 && e < V) {
-                if constexpr (sizeof(T) == 4) u[j] = reinterpret_cast<const unsigned*>(base)[e];
-                else {
-                    const unsigned h = reinterpret_cast<const unsigned short*>(base)[e];
-                    u[j >> 1] = (j & 1) ? ((u[j >> 1] & 0xffffu) | (h << 16)) : ((u[j >> 1] & 0xffff0000u) | h);
-                }
+            const bool in = e >= 0 && e < V;
+            const int64_t at = in ? e : 0;
+            if constexpr (sizeof(T) == 4) c[j] = reinterpret_cast<const unsigned*>(base)[at];
+            else {
+                const unsigned h = reinterpret_cast<const unsigned short*>(base)[at];
+                c[j >> 1] = (j & 1) ? (c[j >> 1] | (h << 16)) : h;
             }
+            constexpr int sh = sizeof(T) == 4 ? 0 : 1;
+            const unsigned mask = sizeof(T) == 4 ? 0xffffffffu : (j & 1) ? 0xffff0000u : 0xffffu;
+            if (in) u[j >> sh] = (u[j >> sh] & ~mask) | (c[j >> sh] & mask);
         }
         return u;
     }
@@ -166,51 +171,137 @@ __device__ __forceinline__ void accumulate(const float* f, float& m, float& s) {
     m = nm;
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int mask) { return __shfl_xor(v, mask, 64); }
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, 0xf, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, ((uint64_t)(unsigned)hi << 32) | (unsigned)lo);
+}
+__device__ __forceinline__ float lane_f32(float v, int l) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+__device__ __forceinline__ double lane_f64(double v, int l) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, l);
+    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), l);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 
-// join over the lanes of groups of W (a power of two <= 64): every lane gets the group's max and fp64 sum
+// a pair (m, s) as it counts under the joint maximum M
+__device__ __forceinline__ double rescaled(float m, double s, float M) {
+    const double r = s * (double)exp_diff_sum(m, finite_or_zero(M));
+    return m > -INFINITY || s != s ? r : 0.0;            // an empty set, or one of -inf only; NaN stays
+}
+// join over groups of W = 4, 16 or 64 consecutive lanes: every lane gets the group's max and sum
 template <int W>
 __device__ __forceinline__ void join_lanes(float& m, double& s) {
     float M = m;
-#pragma unroll
-    for (int d = W / 2; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-    s *= (double)exp_diff_sum(m, finite_or_zero(M));        // m = -inf: the factor is 0, and so is s
-    if (!(m > -INFINITY) && s == s) s = 0.0;            // (-inf) - 0 and an empty set
-#pragma unroll
-    for (int d = W / 2; d >= 1; d >>= 1) s += shfl_xor_f64(s, d);
+    if constexpr (W == 4) {
+        M = fmaxf(M, dpp_row<0xB1>(M));                  // quad_perm [1,0,3,2], [2,3,0,1]
+        M = fmaxf(M, dpp_row<0x4E>(M));
+    } else M = row16_max_dpp(M);
+    if constexpr (W == 64) M = fmaxf(fmaxf(lane_f32(M, 0), lane_f32(M, 16)), fmaxf(lane_f32(M, 32), lane_f32(M, 48)));
+    s = rescaled(m, s, M);
+    if constexpr (W == 4) {
+        s += dpp_f64<0xB1>(s);
+        s += dpp_f64<0x4E>(s);
+    } else {
+        s += dpp_f64<0x128>(s);                          // rotations within rows of 16
+        s += dpp_f64<0x124>(s);
+        s += dpp_f64<0x122>(s);
+        s += dpp_f64<0x121>(s);
+    }
+    if constexpr (W == 64) s = (lane_f64(s, 0) + lane_f64(s, 16)) + (lane_f64(s, 32) + lane_f64(s, 48));
     m = M;
 }
 
 __device__ __forceinline__ int64_t row_action(const RowArgs& a, int64_t row) {
     return a.act64 ? reinterpret_cast<const int64_t*>(a.act)[row] : (int64_t)reinterpret_cast<const int32_t*>(a.act)[row];
 }
+__device__ __forceinline__ int64_t row_group(const RowArgs& a, int64_t row) {      // row / inner; both fit 32 bits
+    return a.one_group ? 0 : (int64_t)((unsigned)row / (unsigned)a.inner);
+}
 __device__ __forceinline__ float row_weight(const RowArgs& a, int64_t row) {
     if (a.pair_w) {
-        const int64_t q = row / a.inner;
+        const int64_t q = row_group(a, row);
         if (a.pair_w[q < a.pairs ? q : q - a.pairs] == 0.0f) return 0.0f;
     }
     return a.w ? a.w[row] : 1.0f;
 }
-__device__ __forceinline__ int64_t row_offset(int64_t row, int64_t inner, int64_t so, int64_t si) {
-    return (row / inner) * so + (row % inner) * si;
+__device__ __forceinline__ int64_t row_offset(const RowArgs& a, int64_t row, int64_t so, int64_t si) {
+    const int64_t q = row_group(a, row);
+    return q * so + (row - q * a.inner) * si;
+}
+
+// Logarithm and exponential in fp64 by their series, to about 1e-14 relative.  One lane of a row evaluates them while the
+// row's other waves wait, so they are short, and their constants are set in scalar registers on the spot (scalar_const;
+// left alone the compiler keeps them in vector registers over the loop of rows: 125 to 155 registers with the library's
+// functions inlined, which halves the waves that hide the loads).
+__device__ __forceinline__ double scalar_const(double c) {
+    asm volatile("" : "+s"(c));
+    return c;
+}
+// log s for s >= 1/2: s = 2^k f, f in [sqrt 1/2, sqrt 2), t = (f - 1) / (f + 1), log f = 2 (t + t^3 / 3 + t^5 / 5 + ...), |t| < 0.172
+__device__ __forceinline__ double log_f64(double s) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, s);
+    int k = (int)(b >> 52) - 1023;
+    double f = __builtin_bit_cast(double, (b & 0x000fffffffffffffull) | 0x3ff0000000000000ull);
+    if (f > scalar_const(1.4142135623730951)) { f *= 0.5; ++k; }
+    const double d = f + 1.0;
+    double r = __builtin_amdgcn_rcp(d);
+    r = fma(r, fma(-d, r, 1.0), r);
+    r = fma(r, fma(-d, r, 1.0), r);
+    const double t = (f - 1.0) * r, w = t * t;
+    double p = scalar_const(1.0 / 15);
+#pragma unroll
+    for (int i = 13; i >= 1; i -= 2) p = fma(p, w, scalar_const(1.0 / i));
+    const double v = fma((double)k, scalar_const(0.6931471805599453), 2.0 * t * p);
+    return s > 0.0 ? v : (s == 0.0 ? -INFINITY : s);            // NaN stays NaN
+}
+// e^x = 2^k (1 + p), p = e^r - 1 by its series, |r| <= log(2) / 2
+__device__ __forceinline__ double exp_parts(double x, int& k) {
+    const double lim = scalar_const(1100.0), c = fmin(fmax(x, -lim), lim), n = rint(c * scalar_const(1.4426950408889634));
+    // log 2 in two words
+    const double r = fma(-n, scalar_const(1.9082149292705877e-10), fma(-n, scalar_const(0.6931471803691238), c));
+    constexpr double fact[13] = {1, 1, 2, 6, 24, 120, 720, 5040, 40320, 362880, 3628800, 39916800, 479001600};
+    double p = scalar_const(1.0 / fact[12]);
+#pragma unroll
+    for (int i = 11; i >= 1; --i) p = fma(p, r, scalar_const(1.0 / fact[i]));
+    k = (int)n;
+    return p * r;
+}
+__device__ __forceinline__ double exp_f64(double x) {
+    int k;
+    const double p = exp_parts(x, k);
+    return x == x ? ldexp(1.0 + p, k) : x;
+}
+__device__ __forceinline__ double expm1_f64(double x) {
+    int k;
+    const double p = exp_parts(x, k);
+    return x == x ? ldexp(p, k) + (ldexp(1.0, k) - 1.0) : x;
 }
 
 // The row's log-probability and, in the policy mode, its loss and coefficient; writes the per-row outputs.
 // L(r) = -min(r A, clip(r, lo, hi) A), r = exp(logp - old);  k = exp(d) - d - 1, d = ref - logp (never negative, 0 at d = 0)
 // d L / d logp = -r A where the unclipped product is the smaller one (or equal), else 0;  d k / d logp = 1 - exp(d)
 template <int MODE>
-__device__ __forceinline__ double row_result(const RowArgs& a, int64_t row, float w, float za, float m, double s,
+__device__ __forceinline__ double row_result(const RowArgs& a, int64_t row, float w, float za, float m, double s, float inv,
                                              float& coef) {
-    const double logp = ((double)za - (double)m) - log(s);
+    const double logp = ((double)za - (double)m) - log_f64(s);
     a.logp[row] = (float)logp;
+    if (MODE == MODE_LOGP && a.logp64) {
+        a.logp64[row] = logp;
+        a.stat_m[row] = m; a.stat_inv[row] = inv;
+    }
     if constexpr (MODE == MODE_POLICY) {
-        const double A = (double)a.adv[row / a.adv_div];
-        const double r = a.old_logp ? exp(logp - (double)a.old_logp[row]) : (logp == logp ? 1.0 : logp);
+        const double A = (double)a.adv[a.adv_div == 1 ? row : a.adv_div == a.inner ? row_group(a, row) : row / a.adv_div];
+        const double r = a.old_logp ? exp_f64(logp - (double)a.old_logp[row]) : (logp == logp ? 1.0 : logp);
         const double un = r * A, cl = fmin(fmax(r, a.clip_lo), a.clip_hi) * A;
         double loss = -(un <= cl ? un : cl), c = un <= cl ? -un : 0.0, k = 0.0;
         if (un != un) loss = c = un;
         if (a.ref_logp) {
-            const double d = (double)a.ref_logp[row] - logp, e = expm1(d);
+            const double d = (double)a.ref_logp[row] - logp, e = expm1_f64(d);
             k = e - d;
             loss += a.kl_coef * k;
             c -= a.kl_coef * e;
@@ -223,6 +314,12 @@ __device__ __forceinline__ double row_result(const RowArgs& a, int64_t row, floa
     return 0.0;
 }
 
+// a workgroup's share of the loss; a launch of one workgroup needs nobody to add them up
+__device__ __forceinline__ void put_loss(const RowArgs& a, double loss) {
+    if (gridDim.x == 1) *a.loss = (float)loss;
+    else a.loss_part[blockIdx.x] = loss;
+}
+
 // outputs of a padding row, and of one whose action does not exist
 template <int MODE>
 __device__ __forceinline__ void row_const(const RowArgs& a, int64_t row, float v) {
@@ -231,13 +328,10 @@ __device__ __forceinline__ void row_const(const RowArgs& a, int64_t row, float v
     if (MODE == MODE_LOGP && a.logp64) a.logp64[row] = (double)v;
 }
 
+// vector v of the gradient: g holds -c p, the action's own element gets its c
 template <typename T>
-__device__ __forceinline__ void grad_vec(const RowView<T>& rv, char* out, bool aligned, int64_t v, const float* f,
-                                         float m, float nci, int64_t a, float coef) {
+__device__ __forceinline__ void put_grad(const RowView<T>& rv, char* out, bool aligned, int64_t v, float* g, int64_t a, float coef) {
     constexpr int VE = Elem<T>::VE;
-    float g[VE];
-#pragma unroll
-    for (int j = 0; j < VE; ++j) g[j] = nci * exp_diff(f[j], m);
     const int64_t ja = a + rv.mis - v * VE;             // the action's place in this vector, if it is here
     if (ja >= 0 && ja < VE)
 #pragma unroll
@@ -254,25 +348,26 @@ __device__ __forceinline__ void fill_row(char* out, int64_t V, float v, int tid,
     for (int64_t i = tid; i < rv.nvec; i += nt) rv.store(out, true, i, f);
 }
 
-// One row per workgroup of NT threads at a time, in KV vectors of registers per thread (KV = 0: streamed twice).
-template <typename T, int NT, int KV, int MODE>
-__global__ __launch_bounds__(NT) void row_kernel(RowArgs a) {
-    constexpr int NW = NT / 64, VE = Elem<T>::VE, U = 4;
-    __shared__ float s_m[NW];
-    __shared__ double s_s[NW];
+// Long rows: RW waves to a row; one row at a time, or four rows to a workgroup where a wave has its own (RW = 1).
+template <typename T, int RW, int U, bool HOLD, int MODE>
+__global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a) {
+    constexpr int NT = RW * 64, RPB = RW == 1 ? 4 : 1, VE = Elem<T>::VE;
+    static_assert(!HOLD || MODE == MODE_POLICY, "only the one-launch gradient keeps a row");
+    __shared__ float s_m[16];
+    __shared__ double s_s[16];
     __shared__ float s_coef;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    double loss = 0.0;                                                    // thread 0's
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = RW == 1 ? lane : threadIdx.x;
+    double loss = 0.0;                                                    // lane 0's of the row's first wave
+    for (int64_t row = (int64_t)blockIdx.x * RPB + (RW == 1 ? wave : 0); row < a.rows; row += (int64_t)gridDim.x * RPB) {
         const float w = row_weight(a, row);
-        char* out = a.dz ? a.dz + row_offset(row, a.inner, a.d_so, a.d_si) * (int64_t)sizeof(T) : nullptr;
+        char* out = a.dz ? a.dz + row_offset(a, row, a.d_so, a.d_si) * (int64_t)sizeof(T) : nullptr;
         int64_t act = -1;
         bool bad = false;
         if (w != 0.0f) {
             act = row_action(a, row);
             bad = act < 0 || act >= a.V;
         }
-        if (w == 0.0f || bad) {                                           // the whole workgroup agrees
+        if (w == 0.0f || bad) {                                           // all of the row's threads agree
             const float v = bad ? NAN : 0.0f;
             if (out) fill_row<T>(out, a.V, v, tid, NT);
             if (tid == 0) {
@@ -281,112 +376,125 @@ __global__ __launch_bounds__(NT) void row_kernel(RowArgs a) {
             }
             continue;
         }
-        const RowView<T> rv(a.z + row_offset(row, a.inner, a.z_so, a.z_si) * (int64_t)sizeof(T), a.V);
+        const RowView<T> rv(a.z + row_offset(a, row, a.z_so, a.z_si) * (int64_t)sizeof(T), a.V);
         const bool aligned = out && (((uintptr_t)out ^ (uintptr_t)rv.base) & 15) == 0;
         float za = 0.0f, m = -INFINITY, inv = 0.0f, coef = 0.0f;
-        u32x4 x[KV > 0 ? KV : 1];
-        if constexpr (KV > 0) {
-#pragma unroll
-            for (int k = 0; k < KV; ++k) {
-                const int64_t v = tid + k * NT;
-                if (v < rv.nvec) x[k] = rv.load(v);
-                else x[k][0] = x[k][1] = x[k][2] = x[k][3] = Elem<T>::NEG_INF;
-            }
-        }
+        float ex[HOLD ? U * VE : 1], lane_m = 0.0f;
         if constexpr (MODE != MODE_GRAD) {
             if (tid == 0) za = Elem<T>::load(rv.base, act);
             float s = 0.0f;
-            if constexpr (KV > 0) {
-                float f[VE];
+            if constexpr (HOLD) {
+                u32x4 y[U];
 #pragma unroll
-                for (int k = 0; k < KV; ++k) {
-                    Elem<T>::unpack(x[k], f);
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) m = fmaxf(m, f[j]);
+                for (int u = 0; u < U; ++u) {
+                    if (tid + u * NT < rv.nvec) y[u] = rv.load(tid + u * NT);
+                    else y[u][0] = y[u][1] = y[u][2] = y[u][3] = Elem<T>::NEG_INF;
                 }
+#pragma unroll
+                for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], ex + u * VE);
+#pragma unroll
+                for (int j = 0; j < U * VE; ++j) m = fmaxf(m, ex[j]);
                 const float ref = finite_or_zero(m);
 #pragma unroll
-                for (int k = 0; k < KV; ++k) {
-                    Elem<T>::unpack(x[k], f);
+                for (int j = 0; j < U * VE; ++j) s += ex[j] = exp_diff_sum(ex[j], ref);
+                lane_m = m;
+            } else for (int64_t v0 = tid; v0 < rv.nvec; v0 += U * NT) {
+                u32x4 y[U];
 #pragma unroll
-                    for (int j = 0; j < VE; ++j) s += exp_diff_sum(f[j], ref);
+                for (int u = 0; u < U; ++u) {
+                    if (v0 + u * NT < rv.nvec) y[u] = rv.load(v0 + u * NT);
+                    else y[u][0] = y[u][1] = y[u][2] = y[u][3] = Elem<T>::NEG_INF;
                 }
-            } else {
-                for (int64_t v0 = tid; v0 < rv.nvec; v0 += U * NT) {
-                    u32x4 y[U];
+                float f[U * VE];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if (v0 + u * NT < rv.nvec) y[u] = rv.load(v0 + u * NT);
-                        else y[u][0] = y[u][1] = y[u][2] = y[u][3] = Elem<T>::NEG_INF;
-                    }
-                    float f[U * VE];
-#pragma unroll
-                    for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], f + u * VE);
-                    accumulate<U * VE>(f, m, s);
-                }
+                for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], f + u * VE);
+                accumulate<U * VE>(f, m, s);
             }
             double sd = (double)s;
             join_lanes<64>(m, sd);
-            if constexpr (NW > 1) {
+            if constexpr (RW > 1) {
                 if (lane == 0) { s_m[wave] = m; s_s[wave] = sd; }
                 __syncthreads();
-                m = lane < NW ? s_m[lane] : -INFINITY;
-                sd = lane < NW ? s_s[lane] : 0.0;
-                join_lanes<NW>(m, sd);
-                m = __shfl(m, 0, 64);
-                sd = __shfl(sd, 0, 64);
+                m = (lane & 15) < RW ? s_m[lane & 15] : -INFINITY;
+                sd = (lane & 15) < RW ? s_s[lane & 15] : 0.0;
+                join_lanes<16>(m, sd);
             }
-            inv = (float)(1.0 / sd);
+            inv = fast_rcp((float)sd);
             if (tid == 0) {
-                loss += row_result<MODE>(a, row, w, za, m, sd, coef);
-                if (MODE == MODE_LOGP && a.logp64) {
-                    a.logp64[row] = ((double)za - (double)m) - log(sd);
-                    a.stat_m[row] = m; a.stat_inv[row] = inv;
-                }
-                s_coef = coef;
+                loss += row_result<MODE>(a, row, w, za, m, sd, inv, coef);
+                if (RW > 1) s_coef = coef;
             }
         } else {
             m = a.stat_m[row]; inv = a.stat_inv[row];
-            coef = w * a.seq_coef[row / a.inner];
+            coef = w * a.seq_coef[row_group(a, row)];
         }
         if (MODE != MODE_LOGP && out) {
-            if constexpr (MODE == MODE_POLICY) { __syncthreads(); coef = s_coef; }
+            if constexpr (MODE == MODE_POLICY) {
+                if constexpr (RW > 1) { __syncthreads(); coef = s_coef; }
+                else coef = lane_f32(coef, 0);
+            }
             const float nci = -coef * inv;
             float f[VE];
-            if constexpr (KV > 0) {
+            if constexpr (HOLD) {
+                const float scale = nci * exp_diff(lane_m, m);
 #pragma unroll
-                for (int k = 0; k < KV; ++k) {
-                    const int64_t v = tid + k * NT;
-                    if (v < rv.nvec) {
-                        Elem<T>::unpack(x[k], f);
-                        grad_vec<T>(rv, out, aligned, v, f, m, nci, act, coef);
+                for (int u = 0; u < U; ++u)
+                    if (tid + u * NT < rv.nvec) {
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) f[j] = scale * ex[u * VE + j];
+                        put_grad<T>(rv, out, aligned, tid + u * NT, f, act, coef);
                     }
-                }
-            } else {
-                for (int64_t v0 = tid; v0 < rv.nvec; v0 += U * NT) {
-                    u32x4 y[U];
+            } else for (int64_t v0 = tid; v0 < rv.nvec; v0 += U * NT) {
+                u32x4 y[U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (v0 + u * NT < rv.nvec) y[u] = rv.load(v0 + u * NT);
+                for (int u = 0; u < U; ++u)
+                    if (v0 + u * NT < rv.nvec) y[u] = rv.load(v0 + u * NT);
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (v0 + u * NT < rv.nvec) {
-                            Elem<T>::unpack(y[u], f);
-                            grad_vec<T>(rv, out, aligned, v0 + u * NT, f, m, nci, act, coef);
-                        }
-                }
+                for (int u = 0; u < U; ++u)
+                    if (v0 + u * NT < rv.nvec) {
+                        Elem<T>::unpack(y[u], f);
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) f[j] = nci * exp_diff(f[j], m);
+                        put_grad<T>(rv, out, aligned, v0 + u * NT, f, act, coef);
+                    }
             }
         }
-        if constexpr (MODE != MODE_GRAD) __syncthreads();   // s_m / s_s / s_coef are free for the next row
+        if constexpr (MODE != MODE_GRAD && RW > 1) __syncthreads();       // s_m / s_s / s_coef are free for the next row
     }
-    if (MODE == MODE_POLICY && tid == 0) a.loss_part[blockIdx.x] = loss;
+    if constexpr (MODE == MODE_POLICY) {
+        if constexpr (RW == 1) {
+            if (lane == 0) s_s[wave] = loss;
+            __syncthreads();
+            loss = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
+        }
+        if (threadIdx.x == 0) put_loss(a, loss);
+    }
 }
 
-// Short rows: G lanes to a row, EPL elements to a lane, 256 / G rows to a workgroup pass.
-template <typename T, int G, int EPL, int MODE>
-__global__ __launch_bounds__(256) void row_lane_kernel(RowArgs a) {
-    __shared__ double s_loss[256 / G];
-    constexpr int RPB = 256 / G;
+// sum over the workgroup in a fixed order, every thread gets it; `red` holds one word per wave
+__device__ __forceinline__ double wave_sum_f64(double s) {
+    s += dpp_f64<0x128>(s);
+    s += dpp_f64<0x124>(s);
+    s += dpp_f64<0x122>(s);
+    s += dpp_f64<0x121>(s);
+    return (lane_f64(s, 0) + lane_f64(s, 16)) + (lane_f64(s, 32) + lane_f64(s, 48));
+}
+__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+    const int nw = blockDim.x >> 6;
+    v = wave_sum_f64(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int i = 0; i < nw; ++i) t += red[i];
+    return t;
+}
+
+// Short rows: G lanes to a row, EPL elements to a lane, NT / G rows to a pass of the workgroup.
+template <typename T, int G, int EPL, int NT, int MODE>
+__global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
+    __shared__ double s_loss[NT / 64];
+    constexpr int RPB = NT / G;
     const int g = threadIdx.x & (G - 1), grp = threadIdx.x / G;
     double loss = 0.0;
     const int64_t step = (int64_t)gridDim.x * RPB, top = (a.rows + RPB - 1) / RPB * RPB;
@@ -396,8 +504,8 @@ __global__ __launch_bounds__(256) void row_lane_kernel(RowArgs a) {
         const float w = in ? row_weight(a, row) : 0.0f;
         const int64_t act = w != 0.0f ? row_action(a, row) : 0;
         const bool bad = act < 0 || act >= a.V, live = w != 0.0f && !bad;
-        const char* z = a.z + row_offset(row, a.inner, a.z_so, a.z_si) * (int64_t)sizeof(T);
-        float x[EPL], m = -INFINITY, inv, coef = 0.0f, za = 0.0f, s = 0.0f;
+        const char* z = a.z + row_offset(a, row, a.z_so, a.z_si) * (int64_t)sizeof(T);
+        float x[EPL], m = -INFINITY, lane_m = 0.0f, inv, coef = 0.0f, za = 0.0f, s = 0.0f;
 #pragma unroll
         for (int k = 0; k < EPL; ++k) {
             x[k] = live && g + k * G < a.V ? Elem<T>::load(z, g + k * G) : -INFINITY;
@@ -406,19 +514,15 @@ __global__ __launch_bounds__(256) void row_lane_kernel(RowArgs a) {
         if constexpr (MODE != MODE_GRAD) {
             if (live) za = Elem<T>::load(z, act);
             const float ref = finite_or_zero(m);
+            lane_m = m;
 #pragma unroll
-            for (int k = 0; k < EPL; ++k) s += exp_diff_sum(x[k], ref);
+            for (int k = 0; k < EPL; ++k) s += x[k] = exp_diff_sum(x[k], ref);
             double sd = (double)s;
             join_lanes<G>(m, sd);
-            inv = (float)(1.0 / sd);
+            inv = fast_rcp((float)sd);
             if (in && g == 0) {
-                if (live) {
-                    loss += row_result<MODE>(a, row, w, za, m, sd, coef);
-                    if (MODE == MODE_LOGP && a.logp64) {
-                        a.logp64[row] = ((double)za - (double)m) - log(sd);
-                        a.stat_m[row] = m; a.stat_inv[row] = inv;
-                    }
-                } else {
+                if (live) loss += row_result<MODE>(a, row, w, za, m, sd, inv, coef);
+                else {
                     row_const<MODE>(a, row, bad ? NAN : 0.0f);
                     if (bad) loss = NAN;
                 }
@@ -426,41 +530,26 @@ __global__ __launch_bounds__(256) void row_lane_kernel(RowArgs a) {
             if constexpr (MODE == MODE_POLICY) coef = __shfl(coef, (threadIdx.x & 63) & ~(G - 1), 64);
         } else {
             m = live ? a.stat_m[row] : 0.0f; inv = live ? a.stat_inv[row] : 0.0f;
-            coef = live ? w * a.seq_coef[row / a.inner] : 0.0f;
+            coef = live ? w * a.seq_coef[row_group(a, row)] : 0.0f;
         }
         if (MODE != MODE_LOGP && in && a.dz) {
-            char* out = a.dz + row_offset(row, a.inner, a.d_so, a.d_si) * (int64_t)sizeof(T);
-            const float nci = -coef * inv;
+            char* out = a.dz + row_offset(a, row, a.d_so, a.d_si) * (int64_t)sizeof(T);
+            float scale = -coef * inv;
+            if (MODE != MODE_GRAD) scale *= exp_diff(lane_m, m);
 #pragma unroll
             for (int k = 0; k < EPL; ++k) {
                 const int64_t e = g + k * G;
                 if (e < a.V) {
-                    const float v = nci * exp_diff(x[k], m) + (e == act ? coef : 0.0f);
+                    const float v = scale * (MODE == MODE_GRAD ? exp_diff(x[k], m) : x[k]) + (e == act ? coef : 0.0f);
                     Elem<T>::store(out, e, live ? v : (bad ? NAN : 0.0f));
                 }
             }
         }
     }
     if constexpr (MODE == MODE_POLICY) {
-        if (g == 0) s_loss[grp] = loss;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            double t = 0.0;
-            for (int i = 0; i < RPB; ++i) t += s_loss[i];
-            a.loss_part[blockIdx.x] = t;
-        }
+        const double t = block_sum_f64(loss, s_loss);                     // lanes other than a row's first hold 0
+        if (threadIdx.x == 0) put_loss(a, t);
     }
-}
-
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
-    const int nw = blockDim.x >> 6;
-    for (int d = 32; d >= 1; d >>= 1) v += shfl_xor_f64(v, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double t = 0.0;
-    for (int i = 0; i < nw; ++i) t += red[i];
-    return t;
 }
 
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const double* __restrict__ part, int64_t n, float* __restrict__ loss) {
@@ -477,77 +566,128 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const double* __restrict
     if (threadIdx.x == 0) *loss = (float)acc;
 }
 
-// One workgroup per pair: the two sequences' weighted sums of log-probabilities, the margin
+// One wave per pair: the two sequences' weighted sums of log-probabilities, the margin
 //   h = beta ((S_c - R_c) - (S_r - R_r)),
 // the pair's loss -(1 - e) log sigmoid(h) - e log sigmoid(-h) and d loss / d S_c = -d loss / d S_r
-//   = beta scale u (e - sigmoid(-h)),  u the pair's weight.
+//   = beta scale u (e - sigmoid(-h)),  u the pair's weight.  A launch of one workgroup walks all pairs and adds the loss up.
 struct PairArgs {
     const double* logp64; const float* w; const float* ref; const float* pair_w;
     int64_t P, T;
     double beta, smooth, scale;
-    float* seq_logp; float* margin; float* seq_coef; double* pair_loss;
+    float* seq_logp; float* margin; float* seq_coef; double* pair_loss; float* loss;
 };
-__global__ __launch_bounds__(256) void pair_kernel(PairArgs a) {
-    __shared__ double red[4];
-    const int64_t p = blockIdx.x;
-    double S[2];
-    for (int side = 0; side < 2; ++side) {
-        const int64_t r0 = (p + side * a.P) * a.T;
-        double acc = 0.0;
-        for (int64_t t = threadIdx.x; t < a.T; t += 256) {
-            const float w = a.w ? a.w[r0 + t] : 1.0f;
-            if (w != 0.0f) acc += (double)w * a.logp64[r0 + t];
+constexpr int PAIR_WAVES = 16;
+__global__ __launch_bounds__(PAIR_WAVES * 64) void pair_kernel(PairArgs a) {
+    __shared__ double red[PAIR_WAVES];
+    const int lane = threadIdx.x & 63;
+    double total = 0.0;
+    for (int64_t p = (int64_t)blockIdx.x * PAIR_WAVES + (threadIdx.x >> 6); p < a.P; p += (int64_t)gridDim.x * PAIR_WAVES) {
+        double S[2];
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const int64_t r0 = (p + side * a.P) * a.T;
+            double acc = 0.0;
+            for (int64_t t0 = lane; t0 < a.T; t0 += 4 * 64) {             // four loads in flight, added in order
+                double v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int64_t t = t0 + 64 * u;
+                    const float w = t < a.T ? (a.w ? a.w[r0 + t] : 1.0f) : 0.0f;
+                    v[u] = t < a.T ? a.logp64[r0 + t] : 0.0;
+                    v[u] = w != 0.0f ? (double)w * v[u] : 0.0;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc += v[u];
+            }
+            S[side] = wave_sum_f64(acc);
         }
-        S[side] = block_sum_f64(acc, red);
+        if (lane == 0) {
+            const double h = a.beta * ((S[0] - (double)a.ref[p]) - (S[1] - (double)a.ref[p + a.P]));
+            const double t = log1p(exp(-fabs(h))), up = t + fmax(-h, 0.0), down = t + fmax(h, 0.0);
+            const double u = a.pair_w ? (double)a.pair_w[p] : 1.0, sw = a.scale * u;
+            const double dn = 1.0 / (1.0 + exp(h));                        // sigmoid(-h)
+            const bool live = u != 0.0;
+            const double c = live ? a.beta * sw * (a.smooth - dn) : 0.0;
+            a.seq_logp[p] = (float)S[0]; a.seq_logp[p + a.P] = (float)S[1];
+            a.margin[p] = live ? (float)h : 0.0f;
+            a.seq_coef[p] = (float)c; a.seq_coef[p + a.P] = (float)-c;
+            double l = sw * ((1.0 - a.smooth) * up + a.smooth * down);
+            if (h != h) l = h * sw;
+            if (!live) l = 0.0;
+            a.pair_loss[p] = l;
+            total += l;
+        }
     }
-    if (threadIdx.x == 0) {
-        const double h = a.beta * ((S[0] - (double)a.ref[p]) - (S[1] - (double)a.ref[p + a.P]));
-        const double t = log1p(exp(-fabs(h))), up = t + fmax(-h, 0.0), down = t + fmax(h, 0.0);
-        const double u = a.pair_w ? (double)a.pair_w[p] : 1.0, sw = a.scale * u;
-        const double dn = 1.0 / (1.0 + exp(h));                            // sigmoid(-h)
-        const bool live = u != 0.0;
-        const double c = live ? a.beta * sw * (a.smooth - dn) : 0.0;
-        a.seq_logp[p] = (float)S[0]; a.seq_logp[p + a.P] = (float)S[1];
-        a.margin[p] = live ? (float)h : 0.0f;
-        a.seq_coef[p] = (float)c; a.seq_coef[p + a.P] = (float)-c;
-        double l = sw * ((1.0 - a.smooth) * up + a.smooth * down);
-        if (h != h) l = h * sw;
-        a.pair_loss[p] = live ? l : 0.0;
+    if (a.loss) {
+        total = block_sum_f64(total, red);
+        if (threadIdx.x == 0) *a.loss = (float)total;
     }
 }
 
 constexpr int64_t MAX_GRID = 16384;
 
 template <typename T, int MODE>
-static int64_t launch_rows(const RowArgs& a, hipStream_t st, bool dry) {
-    constexpr int VE = Elem<T>::VE;
+static int64_t launch_rows(const RowArgs& a, hipStream_t st) {
     int64_t grid;
-#define MCTSQ_ROWS(kernel, nt, per)                                                               \
+#define MCTSQ_ROWS(nt, per, ...)                                                                  \
     do {                                                                                          \
         grid = (a.rows + (per) - 1) / (per);                                                      \
         if (grid > MAX_GRID) grid = MAX_GRID;                                                     \
-        if (!dry) hipLaunchKernelGGL((kernel), dim3((unsigned)grid), dim3(nt), 0, st, a);         \
+        hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)grid), dim3(nt), 0, st, a);              \
         return grid;                                                                              \
     } while (0)
-#define MCTSQ_COMMA ,
-    // nvec <= V / VE + 2 whatever the alignment
-    const int64_t nv = a.V / VE + 2;
-    if (a.V <= 32) MCTSQ_ROWS(row_lane_kernel<T MCTSQ_COMMA 4 MCTSQ_COMMA 8 MCTSQ_COMMA MODE>, 256, 64);
-    if (a.V <= 256) MCTSQ_ROWS(row_lane_kernel<T MCTSQ_COMMA 16 MCTSQ_COMMA 16 MCTSQ_COMMA MODE>, 256, 16);
-    if (nv <= 64 * 4) MCTSQ_ROWS(row_kernel<T MCTSQ_COMMA 64 MCTSQ_COMMA 4 MCTSQ_COMMA MODE>, 64, 1);
-    if (nv <= 256 * 4) MCTSQ_ROWS(row_kernel<T MCTSQ_COMMA 256 MCTSQ_COMMA 4 MCTSQ_COMMA MODE>, 256, 1);
-    if (nv <= 1024 * 4) MCTSQ_ROWS(row_kernel<T MCTSQ_COMMA 1024 MCTSQ_COMMA 4 MCTSQ_COMMA MODE>, 1024, 1);
-    if (nv <= 1024 * 8) MCTSQ_ROWS(row_kernel<T MCTSQ_COMMA 1024 MCTSQ_COMMA 8 MCTSQ_COMMA MODE>, 1024, 1);
-    MCTSQ_ROWS(row_kernel<T MCTSQ_COMMA 1024 MCTSQ_COMMA 0 MCTSQ_COMMA MODE>, 1024, 1);
+    const int64_t bytes = a.V * (int64_t)sizeof(T);
+    if (a.V <= 32) {
+        // up to 1024 rows (the agent's batch) one workgroup takes them all and adds its own loss up: one launch
+        if (MODE == MODE_POLICY && a.rows <= 1024) {
+            hipLaunchKernelGGL((row_lane_kernel<T, 4, 8, 1024, MODE>), dim3(1), dim3(1024), 0, st, a);
+            return 1;
+        }
+        MCTSQ_ROWS(256, 64, row_lane_kernel<T, 4, 8, 256, MODE>);
+    }
+    if (a.V <= 256) MCTSQ_ROWS(256, 16, row_lane_kernel<T, 16, 16, 256, MODE>);
+    // Measured (policy loss, 2 V bytes a bf16 row, 33 to 270 MB of logits; GB/s read + written): waves per row and vectors
+    // per lane so that one row just fits keeps the most rows in flight -- V = 2040 RW 1 U 4 3900 (RW 2 2830), 8184 RW 2 U 8
+    // 4780 (RW 4 3500), 16000 RW 4 U 8 5050 (RW 8 U 4 4340), 65000 RW 16 U 8 4660 (streamed 3880); only 32000 is better
+    // streamed by 8 waves (4150 against 3900) as two held rows are all that fit a CU; fp32 rows hold half as many
+    // values per vector and have no such gap (32000: held 5220, streamed 4560).  131072 streamed by 16 waves 3840.
+    // vectors of a row: at its worst alignment, unless every row starts on a vector
+    const int64_t es = sizeof(T), starts = (int64_t)((uintptr_t)a.z & 15) | ((a.z_si | (a.one_group ? 0 : a.z_so)) * es & 15);
+    const int64_t nv = (a.V + (starts ? 2 * Elem<T>::VE - 2 : Elem<T>::VE - 1)) / Elem<T>::VE;
+    if (nv <= 64) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 1, MODE == MODE_POLICY, MODE>);
+    if (nv <= 128) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 2, MODE == MODE_POLICY, MODE>);
+    if constexpr (MODE == MODE_POLICY) {
+        if (nv <= 256) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, true, MODE>);
+        if (nv <= 512) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 8, true, MODE>);
+        if (nv <= 1024) MCTSQ_ROWS(128, 1, row_kernel<T, 2, 8, true, MODE>);
+        if (nv <= 2048) MCTSQ_ROWS(256, 1, row_kernel<T, 4, 8, true, MODE>);
+        if (nv <= 4096) {
+            if constexpr (sizeof(T) == 4) MCTSQ_ROWS(512, 1, row_kernel<T, 8, 8, true, MODE>);
+            else MCTSQ_ROWS(512, 1, row_kernel<T, 8, 4, false, MODE>);
+        }
+        if (nv <= 8192) MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 8, true, MODE>);
+        MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 4, false, MODE>);
+    } else if constexpr (MODE == MODE_LOGP) {
+        // one pass, few registers: a wave per row up to 16 KB, four above (32000 bf16: 4 waves 5190 GB/s, 16 waves 3480) --
+        // unless there are too few rows to fill the chip that way, when the whole workgroup shortens each (64 rows of
+        // 32000: 10.4 us against 15.7)
+        if (a.rows * (bytes <= 16384 ? 1 : 4) < 2048 && nv > 256) MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 4, false, MODE>);
+        if (bytes <= 16384) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, false, MODE>);
+        MCTSQ_ROWS(256, 1, row_kernel<T, 4, 4, false, MODE>);
+    } else {
+        // statistics are known: a plain sweep
+        if (bytes <= 8192) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, false, MODE>);
+        if (bytes <= 32768) MCTSQ_ROWS(128, 1, row_kernel<T, 2, 4, false, MODE>);
+        MCTSQ_ROWS(512, 1, row_kernel<T, 8, 4, false, MODE>);
+    }
 #undef MCTSQ_ROWS
-#undef MCTSQ_COMMA
 }
 
 template <int MODE>
-static int64_t launch_rows(int dtype, const RowArgs& a, hipStream_t st, bool dry = false) {
-    if (dtype == DT_F32) return launch_rows<float, MODE>(a, st, dry);
-    if (dtype == DT_BF16) return launch_rows<__bf16, MODE>(a, st, dry);
-    return launch_rows<_Float16, MODE>(a, st, dry);
+static int64_t launch_rows(int dtype, const RowArgs& a, hipStream_t st) {
+    if (dtype == DT_F32) return launch_rows<float, MODE>(a, st);
+    if (dtype == DT_BF16) return launch_rows<__bf16, MODE>(a, st);
+    return launch_rows<_Float16, MODE>(a, st);
 }
 
 // shapes and strides every entry point shares; fills the logits part of `a`
@@ -555,6 +695,7 @@ static int fill_rows(RowArgs& a, const void* d_logits, int dtype, int64_t rows, 
                      int64_t stride_inner, int64_t vocab, const void* d_act, int act_bytes, const float* d_weight) {
     MCTSQ_CHECK(dtype >= 0 && dtype <= 2, "logits dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
     MCTSQ_CHECK(rows >= 0 && vocab >= 1 && inner >= 1, "rows must not be negative, vocab and inner at least 1");
+    MCTSQ_CHECK(rows < ((int64_t)1 << 31) && vocab < ((int64_t)1 << 40), "at most 2^31 - 1 rows");
     MCTSQ_CHECK(rows % inner == 0, "rows must be a multiple of the inner extent");
     MCTSQ_CHECK(act_bytes == 4 || act_bytes == 8, "actions must be 4- or 8-byte integers");
     MCTSQ_CHECK(rows == 0 || (d_logits && d_act), "NULL device pointer");
@@ -564,6 +705,7 @@ static int fill_rows(RowArgs& a, const void* d_logits, int dtype, int64_t rows, 
     a = RowArgs{};
     a.z = (const char*)d_logits; a.z_so = stride_outer; a.z_si = stride_inner;
     a.rows = rows; a.inner = inner; a.V = vocab;
+    a.one_group = inner == rows;
     a.act = d_act; a.act64 = act_bytes == 8; a.w = d_weight; a.adv_div = 1;
     return 0;
 }
@@ -632,10 +774,10 @@ extern "C" int mctsq_policy_loss(const void* d_logits, int dtype, int64_t rows, 
         if (d_dlogits) { if (int rc = fill_grad(a, d_dlogits, dtype, dstride_outer, dstride_inner)) return rc; }
         a.old_logp = d_old_logp; a.ref_logp = d_ref_logp; a.adv = d_adv; a.adv_div = adv_div;
         a.clip_lo = 1.0 - clip_low; a.clip_hi = 1.0 + clip_high; a.kl_coef = kl_coef; a.scale = loss_scale;
-        a.logp = d_logp; a.kl = d_kl; a.loss_part = (double*)d_ws;
+        a.logp = d_logp; a.kl = d_kl; a.loss_part = (double*)d_ws; a.loss = d_loss;
         parts = launch_rows<MODE_POLICY>(dtype, a, st);
     }
-    hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)d_ws, parts, d_loss);
+    if (parts != 1) hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)d_ws, parts, d_loss);
     MCTSQ_HIP(hipGetLastError());
     return 0;
 }
@@ -668,22 +810,27 @@ extern "C" int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pa
     a.logp64 = (double*)(ws + off[0]); a.stat_m = (float*)(ws + off[1]); a.stat_inv = (float*)(ws + off[2]);
     a.logp = (float*)(ws + off[3]);
     a.pair_w = d_pair_weight; a.pairs = pairs;
-    if (rows > 0) {
-        if (d_dlogits) { if (int rc = fill_grad(a, d_dlogits, dtype, dstride_outer, dstride_inner)) return rc; }
-        RowArgs f = a;
-        f.dz = nullptr;
-        launch_rows<MODE_LOGP>(dtype, f, st);
-    }
+    if (rows > 0 && d_dlogits) { if (int rc = fill_grad(a, d_dlogits, dtype, dstride_outer, dstride_inner)) return rc; }
+    a.seq_coef = (float*)(ws + off[4]);
     PairArgs p{};
     p.logp64 = a.logp64; p.w = d_weight; p.ref = d_ref_logp; p.pair_w = d_pair_weight; p.P = pairs; p.T = tokens;
     p.beta = beta; p.smooth = label_smoothing; p.scale = loss_scale;
     p.seq_logp = d_seq_logp; p.margin = d_margin; p.seq_coef = (float*)(ws + off[4]); p.pair_loss = (double*)(ws + off[5]);
-    if (pairs > 0) hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pairs), dim3(256), 0, st, p);
-    hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)p.pair_loss, pairs, d_loss);
-    if (rows > 0 && d_dlogits) {
-        a.seq_coef = p.seq_coef;
-        launch_rows<MODE_GRAD>(dtype, a, st);
+    // The gradient reads the logits again, from memory where they are larger than the caches (8 pairs of 102 MB: 398 us at
+    // 5.15 TB/s for two readings and one writing would be 359; pairs sent through in groups of 32 to 224 MB so that the
+    // second reading could find them cached took 485 to 529).
+    if (rows > 0) {
+        RowArgs f = a;
+        f.dz = nullptr;
+        launch_rows<MODE_LOGP>(dtype, f, st);
     }
+    // up to 64 pairs one workgroup walks them and adds the loss up (four pairs to a wave); more are spread, and summed after
+    const bool one = pairs <= 64;
+    const int64_t pg = one ? 1 : (pairs + PAIR_WAVES - 1) / PAIR_WAVES;
+    p.loss = one ? d_loss : nullptr;
+    hipLaunchKernelGGL(pair_kernel, dim3((unsigned)(pg < MAX_GRID ? pg : MAX_GRID)), dim3(PAIR_WAVES * 64), 0, st, p);
+    if (rows > 0 && d_dlogits) launch_rows<MODE_GRAD>(dtype, a, st);
+    if (!one) hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)p.pair_loss, pairs, d_loss);
     MCTSQ_HIP(hipGetLastError());
     return 0;
 }

@@ -14,11 +14,23 @@ current stream of the logits' device; nothing synchronises, scratch comes from t
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ._lib import MctsqError, lib, on_device, ptr, stream_ptr
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@functools.lru_cache(maxsize=256)
+def _policy_ws(n):
+    return lib.check(lib.mctsq_policy_loss_workspace_bytes(n))
+
+
+@functools.lru_cache(maxsize=256)
+def _preference_ws(pairs, tokens):
+    return lib.check(lib.mctsq_preference_loss_workspace_bytes(pairs, tokens))
 
 
 def _rows(logits, actions, what="logits"):
@@ -111,10 +123,11 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, weight=Non
     d = _grad_out(logits, out) if grad else None
     dso, dsi = _out_strides(d) if grad else (0, 0)
     with on_device(dev):
-        need = lib.check(lib.mctsq_policy_loss_workspace_bytes(n))
+        need = _policy_ws(n)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         loss = torch.empty(1, dtype=torch.float32, device=dev)
-        logp, kl = torch.empty((2, *lead), dtype=torch.float32, device=dev)
+        logp = torch.empty(lead, dtype=torch.float32, device=dev)
+        kl = torch.empty(lead, dtype=torch.float32, device=dev)
         lib.check(lib.mctsq_policy_loss(ptr(logits), _DTYPE[logits.dtype], n, inner, so, si, V, ptr(actions),
                                         actions.element_size(), ptr(old_logp), ptr(ref_logp), ptr(advantages), adv_div,
                                         ptr(weight), clip_low, clip_high, kl_coef, loss_scale, ptr(loss), ptr(logp),
@@ -149,7 +162,7 @@ def preference_loss(logits, actions, ref_logp, weight=None, beta=0.1, label_smoo
     d = _grad_out(logits, out) if grad else None
     dso, dsi = _out_strides(d) if grad else (0, 0)
     with on_device(dev):
-        need = lib.check(lib.mctsq_preference_loss_workspace_bytes(P, T))
+        need = _preference_ws(P, T)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         loss = torch.empty(1, dtype=torch.float32, device=dev)
         seq = torch.empty(2 * P, dtype=torch.float32, device=dev)
