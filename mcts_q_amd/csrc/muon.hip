@@ -19,7 +19,10 @@
 // Planes are stored as the matrix instruction's operand fragments, [row tile of 16][k block of 32][lane 64][8], 1 KB in a
 // row per fragment, so a tile is fetched into LDS lane by lane (global_load_lds) and read back without a bank conflict.
 // X is kept both ways (k along m for A, k along n for B X).
+#include <limits.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "device_utils.hpp"
 
@@ -37,7 +40,6 @@ struct MuMat {
     int n, m;                       // working shape, n <= m
     int np, mp;                     // padded to the tile
     int rows, cols;                 // the matrix as the caller has it; transposed when rows > cols
-    int sym0, full0, blk0;          // first tile / tile / 64 x 64 block of this matrix in the launch
     float lrs;                      // learning rate times the shape's factor
     const void* x; int64_t ldx;     // gradient, or the matrix to orthogonalise
     float* mom;                     // momentum [rows][cols], NULL: orthogonalise x
@@ -49,9 +51,18 @@ struct MuArgs {
     int count, xtype, otype;        // element types of x and, when orthogonalising, out
     float mu, decay; int nesterov;
     double eps;
+    int first[MU_GROUP];            // the launch's first workgroup of each matrix (INT_MAX past the last)
     MuMat mat[MU_GROUP];
 };
 static_assert(sizeof(MuArgs) <= 3584, "kernel arguments");
+
+// the matrix that workgroup b belongs to; without an early exit, so that the scalar loads go out together
+__device__ __forceinline__ int mu_which(const MuArgs& a, int b) {
+    int w = -1;
+#pragma unroll
+    for (int i = 0; i < MU_GROUP; ++i) w += a.first[i] <= b;
+    return w;
+}
 
 __device__ __forceinline__ float mu_load(const void* p, int64_t i, int type) {
     if (type == MU_F32) return reinterpret_cast<const float*>(p)[i];
@@ -59,20 +70,49 @@ __device__ __forceinline__ float mu_load(const void* p, int64_t i, int type) {
 }
 
 // ---- momentum and squares ------------------------------------------------------------------------------------------
+__device__ __forceinline__ float4 mu_load4(const void* p, int64_t i, int type) {
+    if (type == MU_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+    const uint2 b = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p) + i);
+    return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
+                       __uint_as_float(b.y & 0xffff0000u));
+}
+__device__ __forceinline__ float mu_update(const MuArgs& a, float g, float& m) {        // new momentum, and u
+    m = fmaf(a.mu, m, g);
+    return a.nesterov ? fmaf(a.mu, m, g) : m;
+}
+
 __global__ __launch_bounds__(256) void mu_norm_kernel(MuArgs a) {
     __shared__ double red[4];
     const MuMat& t = a.mat[blockIdx.y];
-    const int64_t total = (int64_t)t.rows * t.cols;
+    const int64_t total = (int64_t)t.rows * t.cols, tid = (int64_t)blockIdx.x * 256 + threadIdx.x, nt = (int64_t)MU_PARTS * 256;
     double acc = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)MU_PARTS * 256) {
-        const int64_t r = i / t.cols, c = i - r * t.cols;
+    const int xa = a.xtype == MU_F32 ? 15 : 7;
+    const bool flat = t.ldx == t.cols || t.rows == 1;
+    int64_t tail = 0;
+    if (flat && ((uintptr_t)t.x & xa) == 0 && ((uintptr_t)t.mom & 15) == 0) {
+        tail = total & ~(int64_t)3;
+        for (int64_t i = tid * 4; i < tail; i += nt * 4) {
+            const float4 g = mu_load4(t.x, i, a.xtype);
+            float u[4] = {g.x, g.y, g.z, g.w};
+            if (t.mom) {
+                float4 m4 = *reinterpret_cast<const float4*>(t.mom + i);
+                u[0] = mu_update(a, g.x, m4.x); u[1] = mu_update(a, g.y, m4.y);
+                u[2] = mu_update(a, g.z, m4.z); u[3] = mu_update(a, g.w, m4.w);
+                *reinterpret_cast<float4*>(t.mom + i) = m4;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc = fma((double)u[c], (double)u[c], acc);
+        }
+    }
+    for (int64_t i = tail + tid; i < total; i += nt) {
+        const int64_t r = flat ? 0 : i / t.cols, c = i - r * t.cols;
         float u = mu_load(t.x, r * t.ldx + c, a.xtype);
         if (t.mom) {
-            const float m = fmaf(a.mu, t.mom[i], u);
+            float m = t.mom[i];
+            u = mu_update(a, u, m);
             t.mom[i] = m;
-            u = a.nesterov ? fmaf(a.mu, m, u) : m;
         }
-        acc += (double)u * u;
+        acc = fma((double)u, (double)u, acc);
     }
     for (int d = 32; d >= 1; d >>= 1) acc += __shfl_xor(acc, d, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
@@ -80,18 +120,21 @@ __global__ __launch_bounds__(256) void mu_norm_kernel(MuArgs a) {
     if (threadIdx.x == 0) t.part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// |u|_F from the parts (every lane of a wave gets it): up = the power of two that brings it into [1/2, 1), s = the rest
-// of 1 / (|u| + eps)
-__device__ __forceinline__ void mu_scale(const MuMat& t, double eps, double& up, float& s) {
-    double acc = 0.0;
-    for (int i = threadIdx.x & 63; i < MU_PARTS; i += 64) acc += t.part[i];
-    for (int d = 32; d >= 1; d >>= 1) acc += __shfl_xor(acc, d, 64);
-    const double norm = sqrt(acc);
+// From the sum of squares: up = the power of two that brings |u|_F into [1/2, 1), s = the rest of 1 / (|u|_F + eps)
+__device__ __forceinline__ void mu_scale_of(double squares, double eps, double& up, float& s) {
+    const double norm = sqrt(squares);
     int e = 0;
     if (norm > 0.0 && norm < INFINITY) (void)frexp(norm, &e);
     e = e > 600 ? 600 : (e < -600 ? -600 : e);
     up = ldexp(1.0, -e);
     s = (float)(ldexp(1.0, e) / (norm + eps));
+}
+// the same from the parts of mu_norm_kernel; every lane of a wave gets it
+__device__ __forceinline__ void mu_scale(const MuMat& t, double eps, double& up, float& s) {
+    double acc = 0.0;
+    for (int i = threadIdx.x & 63; i < MU_PARTS; i += 64) acc += t.part[i];
+    for (int d = 32; d >= 1; d >>= 1) acc += __shfl_xor(acc, d, 64);
+    mu_scale_of(acc, eps, up, s);
 }
 
 // ---- planes of X_0 and its transpose -----------------------------------------------------------------------------------
@@ -114,32 +157,56 @@ struct MuPlanes {                   // where a matrix's planes are; plane p of X
 template <int P>
 __global__ __launch_bounds__(256) void mu_planes_kernel(MuArgs a) {
     __shared__ float tile[64][65];
-    int w = 0;
-    while (w + 1 < a.count && (int)blockIdx.x >= a.mat[w + 1].blk0) ++w;
+    const int w = mu_which(a, blockIdx.x);
     const MuMat& t = a.mat[w];
-    const int blk = blockIdx.x - t.blk0, nb = t.mp / 64, bi = blk / nb * 64, bj = blk % nb * 64;     // working coordinates
+    const int blk = blockIdx.x - a.first[w], nb = t.mp / 64, bi = blk / nb * 64, bj = blk % nb * 64;     // working coordinates
     const bool tr = t.rows > t.cols;
     double up; float s;
     mu_scale(t, a.eps, up, s);
-    const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
-    for (int y = y0; y < 64; y += 4) {               // x runs along the caller's columns
-        const int r = (tr ? bj : bi) + y, c = (tr ? bi : bj) + x;
-        float u = 0.0f;
-        if (r < t.rows && c < t.cols) {
-            u = mu_load(t.x, r * t.ldx + c, a.xtype);
-            if (t.mom) {
-                const float m = t.mom[(int64_t)r * t.cols + c];
-                u = a.nesterov ? fmaf(a.mu, m, u) : m;
+    {
+        // x runs along the caller's columns, four at a time
+        const int x = (threadIdx.x & 15) * 4, c = (tr ? bi : bj) + x;
+        const bool vec = ((uintptr_t)t.x & (a.xtype == MU_F32 ? 15 : 7)) == 0 && (t.ldx & 3) == 0 && (t.cols & 3) == 0
+                         && ((uintptr_t)t.mom & 15) == 0;
+        const double f = up * (double)PLANE;
+#pragma unroll
+        for (int y = threadIdx.x >> 4; y < 64; y += 16) {
+            const int r = (tr ? bj : bi) + y;
+            float u[4] = {0.f, 0.f, 0.f, 0.f};
+            if (r < t.rows && c < t.cols) {
+                if (vec) {
+                    const float4 g = mu_load4(t.x, r * t.ldx + c, a.xtype);
+                    u[0] = g.x; u[1] = g.y; u[2] = g.z; u[3] = g.w;
+                    if (t.mom) {
+                        const float4 m = *reinterpret_cast<const float4*>(t.mom + (int64_t)r * t.cols + c);
+                        const float mm[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) u[k] = a.nesterov ? fmaf(a.mu, mm[k], u[k]) : mm[k];
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (c + k < t.cols) {
+                            u[k] = mu_load(t.x, r * t.ldx + c + k, a.xtype);
+                            if (t.mom) {
+                                const float m = t.mom[(int64_t)r * t.cols + c + k];
+                                u[k] = a.nesterov ? fmaf(a.mu, m, u[k]) : m;
+                            }
+                        }
+                }
             }
-            u = (float)((double)u * up * (double)PLANE);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float v = (float)((double)u[k] * f);
+                if (tr) tile[x + k][y] = v;
+                else tile[y][x + k] = v;
+            }
         }
-        if (tr) tile[x][y] = u;
-        else tile[y][x] = u;
     }
     __syncthreads();
     const MuPlanes<P> pl(t);
     const int lane = threadIdx.x & 63, row = lane & 15, k0 = (lane >> 4) * 8;
-    for (int f = y0; f < 16; f += 4) {               // 8 fragments of X, 8 of its transpose
+    for (int f = threadIdx.x >> 6; f < 16; f += 4) {  // 8 fragments of X, 8 of its transpose
         const bool T = f >= 8;
         const int rt = (f & 7) >> 1, kb = f & 1;
         f16x8 hi, lo;
@@ -159,183 +226,606 @@ __global__ __launch_bounds__(256) void mu_planes_kernel(MuArgs a) {
 // ---- the products ---------------------------------------------------------------------------------------------------------
 enum { ST_GRAM = 0, ST_POLY = 1, ST_NEXT = 2, ST_LAST = 3 };
 
-// C[i][j] = sum_k R[i][k] S[j][k] over fragments of R and S: a T x T tile, T = 128 or 64, four waves of T/2 x T/2.
-// Two LDS buffers of one k block (32) each; the next block is fetched while the current one is multiplied.
-template <int P, int T>
-__device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, const _Float16* S, int64_t ss, int KB, int ti, int tj,
-                                        f32x4 (&acc)[T / 32][T / 32], _Float16* lds) {
-    constexpr int RT = T / 16, F = 2 * P * RT, W = T / 32;       // row tiles, fragments of a k block, tiles per wave side
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1;
-    auto fetch = [&](int kb, int buf) {
+// tiles of an np x cols product; of a symmetric one the tiles that reach the diagonal or lie below it
+template <int TI, int TJ>
+__host__ __device__ inline int mu_row_tiles(int np, int ti) {
+    const int last = ti * TI + TI < np ? ti * TI + TI : np;              // rows of this tile row end here
+    return (last + TJ - 1) / TJ;
+}
+template <int TI, int TJ>
+__host__ __device__ inline int mu_tiles(int np, int cols, bool sym) {
+    const int nti = (np + TI - 1) / TI;
+    if (!sym) return nti * ((cols + TJ - 1) / TJ);
+    // full tile rows: (ti + 1) TI / TJ tiles each, the last one by its own end
+    return nti * (nti - 1) / 2 * (TI / TJ) + mu_row_tiles<TI, TJ>(np, nti - 1);
+}
+
+// C[i][j] = sum_k R[i][k] S[j][k] over fragments of R and S: a TI x TJ tile by 2 x 2 waves, a k block of 32 at a time.
+// Three LDS buffers: while block k is multiplied from registers, block k + 1 is read from LDS into a second set of registers,
+// blocks k + 2 and k + 3 are on their way from memory.  The buffers are variables of their own, so that the compiler knows that
+// a read of one does not touch what is being fetched into another.
+template <int P, int TI, int TJ>
+struct MuTile {
+    static constexpr int WI = TI / 32, WJ = TJ / 32;                     // 16 x 16 tiles of a wave
+    static constexpr int FI = P * TI / 16, F = FI + P * TJ / 16;         // fragments of a k block: of R, of both
+    static constexpr int L = F / 4;                                      // a wave's share of the fetch
+    static constexpr int BUF = F * FRAG;                                 // halves in a buffer
+    static constexpr int NB = 3;
+    // epilogue: bytes of a 16 x 16 tile in LDS, and how many rows of them fit a wave's half buffer
+    static constexpr int SUB = 1024 + 64;
+    static constexpr int QI = BUF / SUB / WJ >= 4 && WI >= 4 ? 4 : BUF / SUB / WJ >= 2 && WI >= 2 ? 2 : 1;
+    static_assert(QI * WJ * SUB <= BUF && WI % QI == 0, "epilogue");
+    static_assert(F % 4 == 0 && NB * BUF * 2 <= 160 * 1024, "LDS");
+};
+
+template <int P, int TI, int TJ>
+__device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtiles, const _Float16* S, int64_t ss, int stiles,
+                                        int KB, int ti, int tj, f32x4 (&acc)[MuTile<P, TI, TJ>::WI][MuTile<P, TI, TJ>::WJ],
+                                        _Float16* b0, _Float16* b1, _Float16* b2) {
+    using C = MuTile<P, TI, TJ>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave >> 1, wj = wave & 1;
+    const _Float16* src[C::L];                   // this wave's fragments of block 0; rows past the matrix: its last tile again
 #pragma unroll
-        for (int f0 = 0; f0 < F; f0 += 4) {
-            const int f = f0 + wave;
-            const int side = f / (P * RT), p = f / RT % P, rt = f % RT;
-            const _Float16* g = (side ? S + p * ss + ((int64_t)(tj * RT + rt) * KB + kb) * FRAG
-                                      : R + p * rs + ((int64_t)(ti * RT + rt) * KB + kb) * FRAG) + lane * 8;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                             (__attribute__((address_space(3))) void*)(lds + ((int64_t)buf * F + f) * FRAG), 16, 0, 0);
+    for (int l = 0; l < C::L; ++l) {
+        const int f = wave * C::L + l;
+        if (f < C::FI) {
+            const int p = f / (TI / 16), rt = min(ti * (TI / 16) + f % (TI / 16), rtiles - 1);
+            src[l] = R + p * rs + (int64_t)rt * KB * FRAG;
+        } else {
+            const int g = f - C::FI, p = g / (TJ / 16), rt = min(tj * (TJ / 16) + g % (TJ / 16), stiles - 1);
+            src[l] = S + p * ss + (int64_t)rt * KB * FRAG;
         }
+    }
+    auto fetch = [&](int kb, _Float16* buf) {
+        kb = kb < KB ? kb : KB - 1;              // past the end: the last block again, so that the counts below hold
+#pragma unroll
+        for (int l = 0; l < C::L; ++l)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[l] + (int64_t)kb * FRAG + lane * 8),
+                                             (__attribute__((address_space(3))) void*)(buf + (wave * C::L + l) * FRAG), 16, 0, 0);
     };
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    fetch(0, 0);
-    for (int kb = 0; kb < KB; ++kb) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);          // vmcnt(0): this wave's part of block kb has arrived
-        __syncthreads();                             // ... and everyone's; nobody reads the other buffer any more
-        if (kb + 1 < KB) fetch(kb + 1, (kb + 1) & 1);
-        const u32x4* b = reinterpret_cast<const u32x4*>(lds + (int64_t)(kb & 1) * F * FRAG) + lane;
-        u32x4 r[P][W], s[P];
+    struct Frags { u32x4 r[P][C::WI], s[P][C::WJ]; };
+    auto read = [&](Frags& f, const _Float16* buf) {
+        const u32x4* b = reinterpret_cast<const u32x4*>(buf) + lane;
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int i = 0; i < W; ++i) r[p][i] = b[(p * RT + wi * W + i) * 64];
+            for (int i = 0; i < C::WI; ++i) f.r[p][i] = b[(p * (TI / 16) + wi * C::WI + i) * 64];
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int p = 0; p < P; ++p) s[p] = b[(P * RT + p * RT + wj * W + j) * 64];
+            for (int j = 0; j < C::WJ; ++j) f.s[p][j] = b[(C::FI + p * (TJ / 16) + wj * C::WJ + j) * 64];
+    };
+    auto multiply = [&](const Frags& f) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                if constexpr (P == 2) {
-                    acc[i][j] = mfma_h(r[1][i], s[0], acc[i][j]);
-                    acc[i][j] = mfma_h(r[0][i], s[1], acc[i][j]);
-                }
-                acc[i][j] = mfma_h(r[0][i], s[0], acc[i][j]);
+        for (int j = 0; j < C::WJ; ++j) {
+            if constexpr (P == 2) {
+#pragma unroll
+                for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[1][i], f.s[0][j], acc[i][j]);
+#pragma unroll
+                for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[0][i], f.s[1][j], acc[i][j]);
             }
+#pragma unroll
+            for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[0][i], f.s[0][j], acc[i][j]);
         }
+    };
+    // this wave's part of the oldest fetch under way has arrived, its own LDS reads are done; then everyone's are
+    auto arrive = [&]() {
+        __builtin_amdgcn_s_waitcnt((C::L & 15) | (C::L >> 4) << 14 | 0x0070);        // vmcnt(L), lgkmcnt(0)
+        asm volatile("s_barrier" ::: "memory");
+    };
+    // multiply block k (in `cur`), read block k + 1 from `next`, fetch block k + 3 into `free`, which held block k
+    auto step = [&](int k, const Frags& cur, Frags& other, const _Float16* next, _Float16* free) {
+        arrive();
+        fetch(k + 3, free);
+        read(other, next);
+        multiply(cur);
+        constexpr int M = P == 2 ? 3 * C::WI * C::WJ : C::WI * C::WJ, D = P * (C::WI + C::WJ);
+        // reads and fetches go out one by one among the products: in a row they hold the wave up
+        static_assert(D == 2 * C::L, "two reads to a fetch");
+#pragma unroll
+        for (int d = 0; d < C::L; ++d) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, M / D, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, M / D, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, M % D, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < C::WI; ++i)
+#pragma unroll
+        for (int j = 0; j < C::WJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frags x, y;
+    fetch(0, b0);
+    fetch(1, b1);
+    arrive();
+    fetch(2, b2);
+    read(x, b0);
+    int k = 0;
+    for (; k + 6 <= KB; k += 6) {
+        step(k, x, y, b1, b0); step(k + 1, y, x, b2, b1); step(k + 2, x, y, b0, b2);
+        step(k + 3, y, x, b1, b0); step(k + 4, x, y, b2, b1); step(k + 5, y, x, b0, b2);
     }
+    if (k < KB) step(k, x, y, b1, b0);
+    if (k + 1 < KB) step(k + 1, y, x, b2, b1);
+    if (k + 2 < KB) step(k + 2, x, y, b0, b2);
+    if (k + 3 < KB) step(k + 3, y, x, b1, b0);
+    if (k + 4 < KB) step(k + 4, x, y, b2, b1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);          // nothing is under way into this workgroup's LDS when it ends
 }
 
+// four consecutive values along k of one row: stored as hi (and lo), and read back
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 template <int P>
-__device__ __forceinline__ float plane_value(const _Float16* p, int64_t ps, int64_t at) {
-    float v = (float)p[at];
-    if (P == 2) v += (float)p[at + ps];
-    return v * UNPLANE;
-}
-// four values along k of one row (k a multiple of 4)
-template <int P>
-__device__ __forceinline__ void put4(_Float16* p, int64_t ps, int64_t at, const float* v) {
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    f16x4 h, l;
+__device__ __forceinline__ void split4(const float* v, f16x4& h, f16x4& l) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         h[r] = (_Float16)(v[r] * PLANE);
-        l[r] = (_Float16)(v[r] * PLANE - (float)h[r]);
+        l[r] = P == 2 ? (_Float16)(v[r] * PLANE - (float)h[r]) : (_Float16)0.0f;
     }
-    *reinterpret_cast<f16x4*>(p + at) = h;
-    if (P == 2) *reinterpret_cast<f16x4*>(p + at + ps) = l;
 }
 template <int P>
-__device__ __forceinline__ void put1(_Float16* p, int64_t ps, int64_t at, float v) {
-    const _Float16 h = (_Float16)(v * PLANE);
-    p[at] = h;
-    if (P == 2) p[at + ps] = (_Float16)(v * PLANE - (float)h);
+struct Quad4 { f16x4 p[P]; };
+template <int P>
+__device__ __forceinline__ Quad4<P> plane_load(const _Float16* at, int64_t ps) {
+    Quad4<P> q;
+#pragma unroll
+    for (int p = 0; p < P; ++p) q.p[p] = *reinterpret_cast<const f16x4*>(at + p * ps);
+    return q;
+}
+template <int P>
+__device__ __forceinline__ float plane_value(const Quad4<P>& q, int r) {
+    return (P == 2 ? (float)q.p[0][r] + (float)q.p[P - 1][r] : (float)q.p[0][r]) * UNPLANE;
 }
 
-template <int P, int T, int ST>
+// `count` (at most four; four where vec is set) results in a row of the caller's matrix, from column c on
+__device__ __forceinline__ void mu_put(const MuArgs& a, const MuMat& t, int row, int c, const float* v, bool vec, int count = 4) {
+    if (row >= t.rows || c >= t.cols) return;
+    const int64_t at = (int64_t)row * t.ldo + c;
+    const int end = t.cols - c < count ? t.cols - c : count;
+    if (t.mom) {
+        float* p = reinterpret_cast<float*>(t.out) + at;
+        if (vec) {
+            float4 q = *reinterpret_cast<const float4*>(p);
+            q.x = fmaf(q.x, a.decay, -t.lrs * v[0]); q.y = fmaf(q.y, a.decay, -t.lrs * v[1]);
+            q.z = fmaf(q.z, a.decay, -t.lrs * v[2]); q.w = fmaf(q.w, a.decay, -t.lrs * v[3]);
+            *reinterpret_cast<float4*>(p) = q;
+        } else
+#pragma unroll
+            for (int k = 0; k < 4; ++k) if (k < end) p[k] = fmaf(p[k], a.decay, -t.lrs * v[k]);
+    } else if (a.otype == MU_F32) {
+        float* p = reinterpret_cast<float*>(t.out) + at;
+        if (vec) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k) if (k < end) p[k] = v[k];
+    } else {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        __bf16* p = reinterpret_cast<__bf16*>(t.out) + at;
+        bf16x4 q;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = (__bf16)(k < end ? v[k] : 0.0f);
+        if (vec) *reinterpret_cast<bf16x4*>(p) = q;
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k) if (k < end) p[k] = q[k];
+    }
+}
+
+template <int P, int TI, int TJ, int ST>
 __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
-    constexpr int W = T / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * P * (T / 16) * FRAG];
-    const bool sym = ST == ST_GRAM || ST == ST_POLY;
-    int w = 0;
-    while (w + 1 < a.count && (int)blockIdx.x >= (sym ? a.mat[w + 1].sym0 : a.mat[w + 1].full0)) ++w;
+    using C = MuTile<P, TI, TJ>;
+    __shared__ __attribute__((aligned(16))) _Float16 b0[C::BUF], b1[C::BUF], b2[C::BUF];
+    constexpr bool sym = ST == ST_GRAM || ST == ST_POLY;
+    const int w = mu_which(a, blockIdx.x), n = mu_tiles<TI, TJ>(a.mat[w].np, sym ? a.mat[w].np : a.mat[w].mp, sym);
+    // workgroups go round the eight XCDs: of every matrix each XCD gets a run of neighbouring tiles, which share operands
+    // in its L2
+    const int lb = blockIdx.x - a.first[w], q = n >> 3, rest = n & 7, x = lb & 7;
+    const int b = x * q + (x < rest ? x : rest) + (lb >> 3);
     const MuMat& t = a.mat[w];
     const MuPlanes<P> pl(t);
-    const int b = blockIdx.x - (sym ? t.sym0 : t.full0);
     int ti, tj;
-    if (sym) {                       // tile b of the lower triangle, row by row
-        ti = (int)((sqrtf(8.0f * b + 1.0f) - 1.0f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= b) ++ti;
-        while (ti * (ti + 1) / 2 > b) --ti;
-        tj = b - ti * (ti + 1) / 2;
-    } else {
-        ti = b % (t.np / T); tj = b / (t.np / T);
+    {
+        const int nti = (t.np + TI - 1) / TI, ntj = (t.mp + TJ - 1) / TJ;
+        if (sym) {                   // tile row ti has the tiles that reach below the diagonal
+            int c = b;
+            for (ti = 0; c >= mu_row_tiles<TI, TJ>(t.np, ti); ++ti) c -= mu_row_tiles<TI, TJ>(t.np, ti);
+            tj = c;
+        } else {                     // bands of 8 tile rows, column by column
+            const int band = b / (8 * ntj), h = nti - band * 8 < 8 ? nti - band * 8 : 8, c = b - band * 8 * ntj;
+            ti = band * 8 + c % h; tj = c / h;
+        }
     }
-    const int cur = it & 1;
-    f32x4 acc[W][W];
-    if (ST == ST_GRAM) mu_tile<P, T>(pl.X(cur), pl.xs, pl.X(cur), pl.xs, t.mp / 32, ti, tj, acc, lds);
-    else if (ST == ST_POLY) mu_tile<P, T>(pl.A, pl.as, pl.A, pl.as, t.np / 32, ti, tj, acc, lds);
-    else mu_tile<P, T>(pl.B, pl.as, pl.XT(cur), pl.xs, t.np / 32, ti, tj, acc, lds);
+    const int cur = it & 1, nt = t.np / 16, mt = t.mp / 16;
+    f32x4 acc[C::WI][C::WJ];
+    if (ST == ST_GRAM) mu_tile<P, TI, TJ>(pl.X(cur), pl.xs, nt, pl.X(cur), pl.xs, nt, t.mp / 32, ti, tj, acc, b0, b1, b2);
+    else if (ST == ST_POLY) mu_tile<P, TI, TJ>(pl.A, pl.as, nt, pl.A, pl.as, nt, t.np / 32, ti, tj, acc, b0, b1, b2);
+    else mu_tile<P, TI, TJ>(pl.B, pl.as, nt, pl.XT(cur), pl.xs, mt, t.np / 32, ti, tj, acc, b0, b1, b2);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, col = lane & 15;
+    // Lane (quad, col) holds rows 4 quad .. + 3 of column col of every 16 x 16 tile.  The results go through LDS and leave it
+    // in short loops: as they lie they are four neighbours along k of the transposed plane (half a fragment by the wave),
+    // and read eight along a row, two tiles at a time, whole fragments of the plane the other way round.  (Unrolled from the
+    // registers this was 20 to 60 KB of code that every tile runs once, waiting for instructions: 25 to 44 us a tile.)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, col = lane & 15;
     float s = 1.0f;
     if (it == 0 && ST != ST_POLY) { double up; mu_scale(t, a.eps, up, s); }
-    const float unit = UNPLANE * UNPLANE;
+    const float unit = UNPLANE * UNPLANE * (ST == ST_GRAM ? s * s : s);
+    const int lane4 = (col + 16 * (quad >> 1)) * 8 + (quad & 1) * 4;     // this lane's place in a half fragment
+    const int i0 = ti * (TI / 16) + (wave >> 1) * C::WI, j0 = tj * (TJ / 16) + (wave & 1) * C::WJ;
+    // the A that c A^2 is added to: all of this wave's loads at once, as nothing else hides them
+    Quad4<P> old[ST == ST_POLY ? C::WI : 1][C::WJ];
+    if constexpr (ST == ST_POLY)
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+        for (int i = 0; i < C::WI; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const int gi = ti * T + ((wave >> 1) * W + i) * 16 + 4 * q, gj = tj * T + ((wave & 1) * W + j) * 16 + col;
-            float v[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * unit;
-            if constexpr (ST == ST_GRAM) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] *= s * s;
+            for (int j = 0; j < C::WJ; ++j) {
+                const int i16 = min(i0 + i, nt - 1), j16 = min(j0 + j, nt - 1);
+                old[i][j] = plane_load<P>(pl.A + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4, pl.as);
             }
-            if constexpr (ST == ST_POLY) {
+    __syncthreads();                                                     // the operands in LDS are done with
+    // a wave's own 16 x 16 tiles, QI rows of them at a time; 16 bytes after every 16 lanes and every tile starts 16 banks
+    // on, so that neither way of reading runs into bank conflicts
+    char* own = reinterpret_cast<char*>(wave & 1 ? b1 : b0) + (wave >> 1) * C::BUF;          // half a buffer
+    const bool tr = t.rows > t.cols;
+    const bool vec = ST == ST_LAST && (t.ldo & 3) == 0 && (t.cols & 3) == 0 && ((uintptr_t)t.out & (t.mom || a.otype == MU_F32 ? 15 : 7)) == 0;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)              // A is symmetric: its (gj, gi + r) lie side by side
-                    v[r] = fmaf(NS_C, v[r], NS_B * plane_value<P>(pl.A, pl.as, frag_at(gj, gi, t.np) + r));
+    for (int c = 0; c < C::WI; c += C::QI) {
+#pragma unroll
+        for (int q = 0; q < C::QI; ++q)
+#pragma unroll
+            for (int j = 0; j < C::WJ; ++j) {
+                f32x4 v = acc[c + q][j];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] *= unit;
+                    if constexpr (ST == ST_POLY) {                       // A is symmetric: read as it lies, (column, row)
+                        v[r] = fmaf(NS_C, v[r], NS_B * plane_value<P>(old[c + q][j], r));
+                        if (i0 + c + q == j0 + j && 4 * quad + r == col) v[r] += NS_A;
+                    }
+                }
+                *reinterpret_cast<f32x4*>(own + (q * C::WJ + j) * C::SUB + lane * 16 + quad * 16) = v;
             }
-            if constexpr (sym) {
-                _Float16* out = ST == ST_GRAM ? pl.A : pl.B;
-                put4<P>(out, pl.as, frag_at(gj, gi, t.np), v);
-                if (ti != tj)
+        asm volatile("" ::: "memory");           // a wave's LDS accesses are served in order: only the compiler must keep it
+        constexpr int N = C::QI * C::WJ, U = N >= 4 ? 4 : N;             // U tiles' LDS reads under way at once
+        if (ST != ST_LAST || tr)
+            for (int e0 = 0; e0 < N; e0 += U) {
+                f32x4 v4[U];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) put1<P>(out, pl.as, frag_at(gi + r, gj, t.np), v[r]);
-            } else {
+                for (int u = 0; u < U; ++u) v4[u] = *reinterpret_cast<const f32x4*>(own + (e0 + u) * C::SUB + lane * 16 + quad * 16);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    v[r] = s * fmaf(NS_A, plane_value<P>(pl.XT(cur), pl.xs, frag_at(gj, gi, t.np) + r), v[r]);
-                if constexpr (ST == ST_NEXT) {
-                    put4<P>(pl.XT(cur ^ 1), pl.xs, frag_at(gj, gi, t.np), v);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) put1<P>(pl.X(cur ^ 1), pl.xs, frag_at(gi + r, gj, t.mp), v[r]);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (gi + r < t.n && gj < t.m) {
-                            const bool tr = t.rows > t.cols;
-                            const int64_t at = (int64_t)(tr ? gj : gi + r) * t.ldo + (tr ? gi + r : gj);
-                            if (t.mom) {
-                                float* p = reinterpret_cast<float*>(t.out);
-                                p[at] = fmaf(p[at], a.decay, -t.lrs * v[r]);
-                            } else if (a.otype == MU_F32) reinterpret_cast<float*>(t.out)[at] = v[r];
-                            else reinterpret_cast<__bf16*>(t.out)[at] = (__bf16)v[r];
+                for (int u = 0; u < U; ++u) {
+                    const int i16 = i0 + c + (e0 + u) / C::WJ, j16 = j0 + (e0 + u) % C::WJ;
+                    const bool in = i16 < nt && j16 <= (sym ? i16 : mt - 1);
+                    const float v[4] = {v4[u][0], v4[u][1], v4[u][2], v4[u][3]};
+                    if constexpr (ST == ST_LAST) {
+                        if (in) mu_put(a, t, j16 * 16 + col, i16 * 16 + 4 * quad, v, vec);
+                    } else {
+                        f16x4 h, l;
+                        split4<P>(v, h, l);
+                        _Float16* out = (sym ? (ST == ST_GRAM ? pl.A : pl.B) : pl.XT(cur ^ 1))
+                                        + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4;
+                        if (in) {
+                            *reinterpret_cast<f16x4*>(out) = h;
+                            if (P == 2) *reinterpret_cast<f16x4*>(out + (sym ? pl.as : pl.xs)) = l;
                         }
+                    }
                 }
             }
+        constexpr int U2 = N / 2 >= 4 ? 4 : N / 2;
+        if (ST != ST_LAST || !tr)
+            for (int e0 = 0; e0 < N / 2; e0 += U2) {
+                // fragments: row lane & 15, octet lane >> 4 of the 32 columns; the result matrix: four lanes to a row
+                const int row = ST == ST_LAST ? lane >> 2 : lane & 15, oct = ST == ST_LAST ? lane & 3 : lane >> 4;
+                const char* src = own + (2 * e0 + (oct >> 1)) * C::SUB + ((oct & 1) * 8 + 16 * (row >> 2)) * 16 + (row >> 2) * 16 + (row & 3) * 4;
+                float v[U2][8];
+#pragma unroll
+                for (int u = 0; u < U2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[u][k] = *reinterpret_cast<const float*>(src + u * 2 * C::SUB + k * 16);
+#pragma unroll
+                for (int u = 0; u < U2; ++u) {
+                    const int i16 = i0 + c + (e0 + u) / (C::WJ / 2), jp = j0 + (e0 + u) % (C::WJ / 2) * 2;
+                    const bool in = i16 < nt && jp <= (sym ? i16 : mt - 1);
+                    if constexpr (ST == ST_LAST) {
+                        if (in) {
+                            mu_put(a, t, i16 * 16 + row, jp * 16 + oct * 8, v[u], vec);
+                            mu_put(a, t, i16 * 16 + row, jp * 16 + oct * 8 + 4, v[u] + 4, vec);
+                        }
+                    } else {
+                        f16x8 h, l;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            h[k] = (_Float16)(v[u][k] * PLANE);
+                            l[k] = (_Float16)(v[u][k] * PLANE - (float)h[k]);
+                        }
+                        _Float16* out = (sym ? (ST == ST_GRAM ? pl.A : pl.B) : pl.X(cur ^ 1))
+                                        + ((int64_t)i16 * ((sym ? t.np : t.mp) >> 5) + (jp >> 1)) * FRAG + lane * 8;
+                        if (in && (!sym || jp + (lane >> 5) < i16)) {    // on the diagonal the loop above stored the whole tile
+                            *reinterpret_cast<f16x8*>(out) = h;
+                            if (P == 2) *reinterpret_cast<f16x8*>(out + (sym ? pl.as : pl.xs)) = l;
+                        }
+                    }
+                }
+            }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// ---- small matrices: all of it in one workgroup ---------------------------------------------------------------------
+// X and A (then B over A) of one matrix stay in LDS as fragments, 16 waves share the products in blocks of 32 x 32, results
+// wait in registers until everyone has read the operands they replace.  X is kept one way only: where k runs along its rows
+// the fragments are read with the transposing LDS read.  One launch for norm, five steps and update; the launches of the
+// general path cost 60 to 110 us whatever the size (five matrices of 64 x 192 to 128 x 192: 110 us there).
+constexpr int MU_SMALL_LDS = 160 * 1024;
+template <int P> struct MuSmall { static constexpr int NEXT = P == 2 ? 2 : 3, SYM = P == 2 ? 1 : 2; };      // most blocks a wave gets
+
+template <int P> struct MuOperands { u32x4 r[P][2], c[P][2]; };
+// k blocks one after the other, the next one's operands read while the current one is multiplied
+template <int P, typename Load, typename Multiply>
+__device__ __forceinline__ void mu_blocks(int K, const Load& load, const Multiply& multiply) {
+    MuOperands<P> x, y;
+    load(x, 0);
+#pragma unroll 1
+    for (int k = 0; k < K; k += 2) {
+        load(y, k + 1 < K ? k + 1 : k);
+        multiply(x);
+        if (k + 1 == K) break;
+        load(x, k + 2 < K ? k + 2 : k);
+        multiply(y);
+    }
+}
+
+static bool mu_is_small(int64_t rows, int64_t cols, int P) {
+    const int64_t n = round_up(rows < cols ? rows : cols, 32), m = round_up(rows < cols ? cols : rows, 32);
+    const int64_t ni = n / 32, mi = m / 32;
+    return 2 * P * (n * m + n * n) <= MU_SMALL_LDS && ni * mi <= 16 * (P == 2 ? MuSmall<2>::NEXT : MuSmall<1>::NEXT)
+           && ni * (ni + 1) / 2 <= 16 * (P == 2 ? MuSmall<2>::SYM : MuSmall<1>::SYM);
+}
+
+template <int P>
+__global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
+    __shared__ __attribute__((aligned(16))) _Float16 lds[MU_SMALL_LDS / 2];
+    const MuMat& t = a.mat[blockIdx.x];
+    int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int np = (t.n + 31) & ~31, mp = (t.m + 31) & ~31, nb = np / 32, mb = mp / 32;
+    const int xs = np * mp, as = np * np;                 // a plane's halves
+    _Float16 *X = lds, *A = lds + P * xs;
+    const bool tr = t.rows > t.cols;
+
+    // momentum, norm; X's planes cleared meanwhile (padding stays 0)
+    for (int i = threadIdx.x; i < P * xs / 8; i += 1024) reinterpret_cast<u32x4*>(X)[i] = u32x4{0, 0, 0, 0};
+    // A wave takes every 16th row, a lane its columns: nothing to divide, rows' addresses are scalar.  Four rows under way at
+    // once: one workgroup has nobody else to wait with.
+    constexpr int U = 4;
+    double acc64 = 0.0;
+    for (int r0 = wave; r0 < t.rows; r0 += 16 * U)
+        for (int c = lane; c < t.cols; c += 64) {
+            float g[U], m[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = min(r0 + 16 * u, t.rows - 1);
+                g[u] = mu_load(t.x, r * t.ldx + c, a.xtype);
+                m[u] = t.mom ? t.mom[r * t.cols + c] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r0 + 16 * u >= t.rows) continue;
+                float v = g[u];
+                if (t.mom) {
+                    v = mu_update(a, g[u], m[u]);
+                    t.mom[(r0 + 16 * u) * t.cols + c] = m[u];
+                }
+                acc64 = fma((double)v, (double)v, acc64);
+            }
         }
+    for (int d = 32; d >= 1; d >>= 1) acc64 += __shfl_xor(acc64, d, 64);
+    double* red = reinterpret_cast<double*>(A);
+    if (lane == 0) red[wave] = acc64;
+    __syncthreads();
+    double sum = 0.0;
+    for (int i = 0; i < 16; ++i) sum += red[i];
+    double up; float s;
+    mu_scale_of(sum, a.eps, up, s);
+    // up * 2^14 as two fp32 powers of two: the product is exact wherever it matters (below 2^-126 nothing is left of it)
+    int e = (int)(__builtin_bit_cast(uint64_t, up) >> 52) - 1023 + 14;
+    e = e < -250 ? -250 : (e > 250 ? 250 : e);
+    const float f0 = pow2i(e >> 1), f1 = pow2i(e - (e >> 1));
+    for (int r0 = wave; r0 < t.rows; r0 += 16 * U)
+        for (int c = lane; c < t.cols; c += 64) {
+            float g[U], m[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = min(r0 + 16 * u, t.rows - 1);
+                g[u] = mu_load(t.x, r * t.ldx + c, a.xtype);
+                m[u] = t.mom ? t.mom[r * t.cols + c] : 0.0f;             // written by this thread above
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + 16 * u;
+                if (r >= t.rows) continue;
+                const float w = !t.mom ? g[u] : a.nesterov ? fmaf(a.mu, m[u], g[u]) : m[u], v = w * f0 * f1;
+                const int row = tr ? c : r, k = tr ? r : c;
+                _Float16* o = X + ((row >> 4) * mb + (k >> 5)) * FRAG + (((row & 15) + 16 * ((k & 31) >> 3)) << 3) + (k & 7);
+                const _Float16 h = (_Float16)v;
+                o[0] = h;
+                if (P == 2) o[xs] = (_Float16)(v - (float)h);
+            }
+        }
+    __syncthreads();
+
+    const int sym = nb * (nb + 1) / 2, full = nb * mb;
+    // fragment (row tile, k block) of a plane whose k extent is K blocks
+    auto frag = [&](const _Float16* p, int rt, int kb, int K) {
+        return *reinterpret_cast<const u32x4*>(p + (rt * K + kb) * FRAG + lane * 8);
+    };
+    // rows j = 16 jt .. + 15, k = 32 ib .. + 31 of X transposed: groups of 16 lanes read four rows of 16 and get columns
+    auto frag_tr = [&](const _Float16* p, int jt, int ib) {
+        const int g = lane & 15, j = jt * 16 + (g & 3) * 4, rt = 2 * ib + (lane >> 5);
+        const _Float16* at = p + (rt * mb + (j >> 5)) * FRAG + ((((lane >> 4) & 1) * 8 + (g >> 2)) + 16 * ((j & 31) >> 3)) * 8 + (j & 7);
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        union { s16x4 h[2]; u32x4 u; } r;
+        r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+        r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 4 * 8));
+        return r.u;
+    };
+    // lower-triangle block b of the symmetric products
+    auto block = [&](int b, int& bi, int& bj) {
+        for (bi = 0; b > bi; ++bi) b -= bi + 1;
+        bj = b;
+    };
+#pragma unroll 1
+    for (int it = 0; it < 5; ++it) {
+        asm volatile("" : "+v"(lane));           // addresses are made anew: kept over the steps they spill
+        const float sc = it == 0 ? s : 1.0f;
+#pragma unroll 1
+        for (int st = ST_GRAM; st <= ST_POLY; ++st) {     // A = X X^T, then B = a + b A + c A^2 over it
+            const _Float16* src = st == ST_GRAM ? X : A;
+            const int64_t ps = st == ST_GRAM ? xs : as;
+            const int K = st == ST_GRAM ? mb : nb;
+            f32x4 acc[MuSmall<P>::SYM][2][2];
+#pragma unroll
+            for (int q = 0; q < MuSmall<P>::SYM; ++q) {
+                const int b = wave + 16 * q;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (b >= sym) continue;
+                int bi, bj;
+                block(b, bi, bj);
+                auto load = [&](MuOperands<P>& o, int k) {
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            o.r[p][e] = frag(src + p * ps, 2 * bi + e, k, K);
+                            o.c[p][e] = frag(src + p * ps, 2 * bj + e, k, K);
+                        }
+                };
+                mu_blocks<P>(K, load, [&](const MuOperands<P>& o) {
+                    if constexpr (P == 2) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[1][e >> 1], o.c[0][e & 1], acc[q][e >> 1][e & 1]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[0][e >> 1], o.c[1][e & 1], acc[q][e >> 1][e & 1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[0][e >> 1], o.c[0][e & 1], acc[q][e >> 1][e & 1]);
+                });
+                const float unit = UNPLANE * UNPLANE * (st == ST_GRAM ? sc * sc : 1.0f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i16 = 2 * bi + (e >> 1), j16 = 2 * bj + (e & 1);
+                    f32x4& v = acc[q][e >> 1][e & 1];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] *= unit;
+                    if (st == ST_POLY) {
+                        const Quad4<P> o = plane_load<P>(A + frag_at(j16 * 16 + (lane & 15), i16 * 16 + (lane >> 4) * 4, np), as);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            v[x] = fmaf(NS_C, v[x], NS_B * plane_value<P>(o, x));
+                            if (i16 == j16 && (lane >> 4) * 4 + x == (lane & 15)) v[x] += NS_A;
+                        }
+                    }
+                }
+            }
+            __syncthreads();                              // everyone has read A
+#pragma unroll
+            for (int q = 0; q < MuSmall<P>::SYM; ++q) {
+                const int b = wave + 16 * q;
+                if (b >= sym) continue;
+                int bi, bj;
+                block(b, bi, bj);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i16 = 2 * bi + (e >> 1), j16 = 2 * bj + (e & 1);
+                    if (j16 > i16) continue;
+                    const float v[4] = {acc[q][e >> 1][e & 1][0], acc[q][e >> 1][e & 1][1], acc[q][e >> 1][e & 1][2], acc[q][e >> 1][e & 1][3]};
+                    f16x4 h, l;
+                    split4<P>(v, h, l);
+                    _Float16* o = A + frag_at(j16 * 16 + (lane & 15), i16 * 16 + (lane >> 4) * 4, np);
+                    *reinterpret_cast<f16x4*>(o) = h;
+                    if (P == 2) *reinterpret_cast<f16x4*>(o + as) = l;
+                    if (i16 != j16) {
+                        o = A + frag_at(i16 * 16 + (lane >> 4) * 4, j16 * 16 + (lane & 15), np);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {     // rows 8 halves apart
+                            o[x * 8] = h[x];
+                            if (P == 2) o[x * 8 + as] = l[x];
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        // X <- B X; the instruction's rows are X's columns, so that a lane ends with four neighbours of one row
+        f32x4 acc[MuSmall<P>::NEXT][2][2];
+#pragma unroll
+        for (int q = 0; q < MuSmall<P>::NEXT; ++q) {
+            const int b = wave + 16 * q, bi = b % nb, bj = b / nb;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (b >= full) continue;
+            auto load = [&](MuOperands<P>& o, int k) {
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        o.r[p][e] = frag(A + p * as, 2 * bi + e, k, nb);
+                        o.c[p][e] = frag_tr(X + p * xs, 2 * bj + e, k);
+                    }
+            };
+            mu_blocks<P>(nb, load, [&](const MuOperands<P>& o) {
+                if constexpr (P == 2) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[0][e & 1], o.r[1][e >> 1], acc[q][e >> 1][e & 1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[1][e & 1], o.r[0][e >> 1], acc[q][e >> 1][e & 1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[0][e & 1], o.r[0][e >> 1], acc[q][e >> 1][e & 1]);
+            });
+        }
+        __syncthreads();                                  // everyone has read X
+        const bool vec = (t.ldo & 3) == 0 && (t.cols & 3) == 0 && ((uintptr_t)t.out & (t.mom || a.otype == MU_F32 ? 15 : 7)) == 0;
+#pragma unroll
+        for (int q = 0; q < MuSmall<P>::NEXT; ++q) {
+            const int b = wave + 16 * q, bi = b % nb, bj = b / nb;
+            if (b >= full) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int gi = (2 * bi + (e >> 1)) * 16 + (lane & 15), gj = (2 * bj + (e & 1)) * 16 + (lane >> 4) * 4;
+                float v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] = acc[q][e >> 1][e & 1][x] * (UNPLANE * UNPLANE * sc);
+                if (it < 4) {
+                    f16x4 h, l;
+                    split4<P>(v, h, l);
+                    _Float16* o = X + frag_at(gi, gj, mp);
+                    *reinterpret_cast<f16x4*>(o) = h;
+                    if (P == 2) *reinterpret_cast<f16x4*>(o + xs) = l;
+                } else if (!tr) mu_put(a, t, gi, gj, v, vec);
+                else
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) mu_put(a, t, gj + x, gi, v + x, false, 1);
+            }
+        }
+        __syncthreads();
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-struct MuPlan { int T; int64_t bytes; };
+constexpr int MU_PAD = 64;          // sides are padded to this; larger tiles repeat the last rows and drop them
 
-static int64_t mu_planes_halves(int64_t n, int64_t m, int T, int P) {
-    const int64_t np = round_up(n, T), mp = round_up(m, T);
-    return P * (4 * np * mp + 2 * np * np);
-}
-// The tile of a group: 128 unless the launch would then leave CUs without a tile.
-static int mu_tile_size(const mctsq_muon_matrix* mats, int count) {
-    int64_t tiles = 0;
-    for (int i = 0; i < count; ++i) {
-        const int64_t n = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols;
-        const int64_t t = (n + 127) / 128;
-        tiles += t * (t + 1) / 2;
-    }
-    return tiles >= 256 ? 128 : 64;
+static int64_t mu_matrix_bytes(int64_t rows, int64_t cols, int P) {
+    const int64_t n = rows < cols ? rows : cols, m = rows < cols ? cols : rows;
+    const int64_t np = round_up(n, MU_PAD), mp = round_up(m, MU_PAD);
+    return round_up(2 * P * (4 * np * mp + 2 * np * np), 256) + MU_PARTS * 8;
 }
 static int64_t mu_group_bytes(const mctsq_muon_matrix* mats, int count, int P) {
-    const int T = mu_tile_size(mats, count);
     int64_t o = 0;
-    for (int i = 0; i < count; ++i) {
-        const int64_t n = mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols;
-        const int64_t m = mats[i].rows < mats[i].cols ? mats[i].cols : mats[i].rows;
-        o += round_up(mu_planes_halves(n, m, T, P) * 2, 256) + MU_PARTS * 8;
-    }
+    for (int i = 0; i < count; ++i) o += mu_matrix_bytes(mats[i].rows, mats[i].cols, P);
     return o;
 }
 static int mu_check_shapes(const mctsq_muon_matrix* mats, int64_t count) {
@@ -355,44 +845,95 @@ static int64_t mu_bytes(const mctsq_muon_matrix* mats, int64_t count, int P) {
     return need < 256 ? 256 : need;
 }
 
-template <int P, int T>
-static void mu_launch(const MuArgs& a, int sym, int full, int blk, hipStream_t st) {
+// One product stage as tiles of TI x TJ: workgroups, and an estimate of its time in us from what was measured (CUs work off
+// `load` tiles each; a k block takes `step`, a tile's start and end `over`; up to `share` workgroups share a CU's pauses)
+template <int TI, int TJ>
+static double mu_stage(MuArgs& a, bool sym, bool gram, double step, double over, int share, int& tiles) {
+    tiles = 0;
+    double work = 0.0;
+    for (int i = 0; i < MU_GROUP; ++i) {
+        a.first[i] = i < a.count ? tiles : INT_MAX;
+        if (i >= a.count) continue;
+        const int n = mu_tiles<TI, TJ>(a.mat[i].np, sym ? a.mat[i].np : a.mat[i].mp, sym);
+        tiles += n;
+        work += (double)n * ((gram ? a.mat[i].mp : a.mat[i].np) / 32);
+    }
+    const int load = (tiles + 255) / 256;
+    return work / tiles * step * load + over * ((load + share - 1) / share);
+}
+template <int P, int ST>
+static void mu_product(MuArgs& a, int it, hipStream_t st) {
+    constexpr bool sym = ST == ST_GRAM || ST == ST_POLY, gram = ST == ST_GRAM;
+    // fp32: 256 x 128 tiles 0.87 us a k block (0.73 at the matrix pipe's rate) and 23 a tile, 128 x 128 0.50 and 15, 64 x 64
+    // 0.20 and 8 with three to a CU; bf16: 0.33 / 15, 0.19 / 8, 0.10 / 5
+    static constexpr double STEP[2][3] = {{0.33, 0.19, 0.10}, {0.87, 0.50, 0.20}}, OVER[2][3] = {{15, 8, 5}, {23, 15, 8}};
+    int tiles;
+    const double t256 = mu_stage<256, 128>(a, sym, gram, STEP[P - 1][0], OVER[P - 1][0], 1, tiles);
+    const double t128 = mu_stage<128, 128>(a, sym, gram, STEP[P - 1][1], OVER[P - 1][1], P == 2 ? 1 : 2, tiles);
+    const double t64 = mu_stage<64, 64>(a, sym, gram, STEP[P - 1][2], OVER[P - 1][2], 3, tiles);      // a.first as for 64 x 64
+    if (t64 <= t128 && t64 <= t256) {
+        hipLaunchKernelGGL((mu_product_kernel<P, 64, 64, ST>), dim3(tiles), dim3(256), 0, st, a, it);
+    } else if (t128 <= t256) {
+        mu_stage<128, 128>(a, sym, gram, 0, 0, 1, tiles);
+        hipLaunchKernelGGL((mu_product_kernel<P, 128, 128, ST>), dim3(tiles), dim3(256), 0, st, a, it);
+    } else {
+        mu_stage<256, 128>(a, sym, gram, 0, 0, 1, tiles);
+        hipLaunchKernelGGL((mu_product_kernel<P, 256, 128, ST>), dim3(tiles), dim3(256), 0, st, a, it);
+    }
+}
+template <int P>
+static void mu_launch(MuArgs& a, hipStream_t st) {
+    bool small = true;
+    for (int i = 0; i < a.count; ++i) small = small && mu_is_small(a.mat[i].rows, a.mat[i].cols, P);
+    if (small) {
+        hipLaunchKernelGGL(mu_small_kernel<P>, dim3(a.count), dim3(1024), 0, st, a);
+        return;
+    }
     hipLaunchKernelGGL(mu_norm_kernel, dim3(MU_PARTS, a.count), dim3(256), 0, st, a);
+    int blk = 0;
+    for (int i = 0; i < MU_GROUP; ++i) {
+        a.first[i] = i < a.count ? blk : INT_MAX;
+        if (i < a.count) blk += (a.mat[i].np / 64) * (a.mat[i].mp / 64);
+    }
     hipLaunchKernelGGL(mu_planes_kernel<P>, dim3(blk), dim3(256), 0, st, a);
     for (int it = 0; it < 5; ++it) {
-        hipLaunchKernelGGL((mu_product_kernel<P, T, ST_GRAM>), dim3(sym), dim3(256), 0, st, a, it);
-        hipLaunchKernelGGL((mu_product_kernel<P, T, ST_POLY>), dim3(sym), dim3(256), 0, st, a, it);
-        if (it < 4) hipLaunchKernelGGL((mu_product_kernel<P, T, ST_NEXT>), dim3(full), dim3(256), 0, st, a, it);
-        else hipLaunchKernelGGL((mu_product_kernel<P, T, ST_LAST>), dim3(full), dim3(256), 0, st, a, it);
+        mu_product<P, ST_GRAM>(a, it, st);
+        mu_product<P, ST_POLY>(a, it, st);
+        if (it < 4) mu_product<P, ST_NEXT>(a, it, st);
+        else mu_product<P, ST_LAST>(a, it, st);
     }
 }
 
 static int mu_run(const mctsq_muon_matrix* mats, int64_t count, int P, MuArgs& a, double lr, int adjust, char* ws, hipStream_t st) {
     for (int64_t g = 0; g < count; g += MU_GROUP) {
         const int c = (int)(count - g < MU_GROUP ? count - g : MU_GROUP);
-        const int T = mu_tile_size(mats + g, c);
-        int64_t o = 0, sym = 0, full = 0, blk = 0;
+        int64_t o = 0, blk = 0;
         a.count = c;
+        int order[MU_GROUP];                              // longest products first: the short ones fill the gaps at the end
+        for (int i = 0; i < c; ++i) order[i] = i;
+        std::sort(order, order + c, [&](int x, int y) {
+            const int64_t lx = std::max(mats[g + x].rows, mats[g + x].cols), ly = std::max(mats[g + y].rows, mats[g + y].cols);
+            return lx != ly ? lx > ly : x < y;
+        });
         for (int i = 0; i < c; ++i) {
-            const mctsq_muon_matrix& s = mats[g + i];
+            const mctsq_muon_matrix& s = mats[g + order[i]];
             MuMat& t = a.mat[i];
             t = MuMat{};
             t.rows = (int)s.rows; t.cols = (int)s.cols;
             t.n = t.rows < t.cols ? t.rows : t.cols; t.m = t.rows < t.cols ? t.cols : t.rows;
-            t.np = (int)round_up(t.n, T); t.mp = (int)round_up(t.m, T);
+            t.np = (int)round_up(t.n, MU_PAD); t.mp = (int)round_up(t.m, MU_PAD);
             t.x = s.d_x; t.ldx = s.ldx; t.mom = s.d_momentum; t.out = s.d_out; t.ldo = s.ldo;
             const double r = (double)s.rows, k = (double)s.cols;
             t.lrs = (float)(lr * (adjust == MCTSQ_MUON_SPECTRAL ? sqrt(r > k ? r / k : 1.0)
                                   : adjust == MCTSQ_MUON_RMS ? 0.2 * sqrt(r > k ? r : k) : 1.0));
-            t.ws = (_Float16*)(ws + o); o += round_up(mu_planes_halves(t.n, t.m, T, P) * 2, 256);
-            t.part = (double*)(ws + o); o += MU_PARTS * 8;
-            t.sym0 = (int)sym; t.full0 = (int)full; t.blk0 = (int)blk;
-            const int64_t nt = t.np / T;
-            sym += nt * (nt + 1) / 2; full += nt * (t.mp / T); blk += (int64_t)(t.np / 64) * (t.mp / 64);
+            t.ws = (_Float16*)(ws + o);
+            o += mu_matrix_bytes(s.rows, s.cols, P);
+            t.part = (double*)(ws + o) - MU_PARTS;
+            blk += (int64_t)(t.np / 64) * (t.mp / 64);
         }
         MCTSQ_CHECK(blk < ((int64_t)1 << 31), "the matrices of one group are too large");
-        if (P == 2) { if (T == 128) mu_launch<2, 128>(a, sym, full, blk, st); else mu_launch<2, 64>(a, sym, full, blk, st); }
-        else { if (T == 128) mu_launch<1, 128>(a, sym, full, blk, st); else mu_launch<1, 64>(a, sym, full, blk, st); }
+        if (P == 2) mu_launch<2>(a, st);
+        else mu_launch<1>(a, st);
         MCTSQ_HIP(hipGetLastError());
     }
     return 0;
