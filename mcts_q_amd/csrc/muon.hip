@@ -137,21 +137,18 @@ __device__ __forceinline__ void mu_scale(const MuMat& t, double eps, double& up,
     mu_scale_of(acc, eps, up, s);
 }
 
-// ---- planes of X_0 and its transpose -----------------------------------------------------------------------------------
+// ---- planes of X_0 -----------------------------------------------------------------------------------
 // element (row, k) of a plane of K columns
 __device__ __forceinline__ int64_t frag_at(int row, int k, int K) {
     return ((int64_t)(row >> 4) * (K >> 5) + (k >> 5)) * FRAG + (((row & 15) + 16 * ((k & 31) >> 3)) << 3) + (k & 7);
 }
 template <int P>
-struct MuPlanes {                   // where a matrix's planes are; plane p of X starts p * np * mp behind X
-    int64_t xs, as;
-    _Float16 *base, *A, *B;
-    __device__ MuPlanes(const MuMat& t) {
-        xs = (int64_t)t.np * t.mp; as = (int64_t)t.np * t.np;
-        base = t.ws; A = base + 4 * P * xs; B = A + P * as;
-    }
+struct MuPlanes {                   // where a matrix's planes are: X twice (old and new), four n x n matrices
+    int64_t xs, as;                 // halves from a plane to the next
+    _Float16* base;
+    __device__ MuPlanes(const MuMat& t) : xs((int64_t)t.np * t.mp), as((int64_t)t.np * t.np), base(t.ws) {}
     __device__ _Float16* X(int cur) const { return base + cur * P * xs; }
-    __device__ _Float16* XT(int cur) const { return base + (2 + cur) * P * xs; }
+    __device__ _Float16* N(int i) const { return base + 2 * P * xs + i * P * as; }
 };
 
 template <int P>
@@ -206,25 +203,32 @@ __global__ __launch_bounds__(256) void mu_planes_kernel(MuArgs a) {
     __syncthreads();
     const MuPlanes<P> pl(t);
     const int lane = threadIdx.x & 63, row = lane & 15, k0 = (lane >> 4) * 8;
-    for (int f = threadIdx.x >> 6; f < 16; f += 4) {  // 8 fragments of X, 8 of its transpose
-        const bool T = f >= 8;
-        const int rt = (f & 7) >> 1, kb = f & 1;
+#pragma unroll
+    for (int f = threadIdx.x >> 6; f < 8; f += 4) {
+        const int rt = f >> 1, kb = f & 1;
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int i = rt * 16 + row, k = kb * 32 + k0 + e;
-            const float v = T ? tile[k][i] : tile[i][k];
+            const float v = tile[rt * 16 + row][kb * 32 + k0 + e];
             hi[e] = (_Float16)v;
             lo[e] = (_Float16)(v - (float)hi[e]);
         }
-        _Float16* dst = (T ? pl.XT(0) + frag_at(bj + rt * 16, bi + kb * 32, t.np) : pl.X(0) + frag_at(bi + rt * 16, bj + kb * 32, t.mp)) + lane * 8;
+        _Float16* dst = pl.X(0) + frag_at(bi + rt * 16, bj + kb * 32, t.mp) + lane * 8;
         *reinterpret_cast<f16x8*>(dst) = hi;
         if (P == 2) *reinterpret_cast<f16x8*>(dst + pl.xs) = lo;
     }
 }
 
 // ---- the products ---------------------------------------------------------------------------------------------------------
-enum { ST_GRAM = 0, ST_POLY = 1, ST_NEXT = 2, ST_LAST = 3 };
+// ST_SYM: a product of two n x n symmetric matrices that commute, or X X^T: symmetric.  ST_POLY: a + b A + c A^2.
+// ST_NEXT: X <- N X.  ST_LAST: the same into the caller's matrix.
+enum { ST_SYM = 0, ST_POLY = 1, ST_NEXT = 2, ST_LAST = 3 };
+struct MuStage {
+    int r, s, out;                  // the n x n matrices R, S and the result; r = -1: X X^T
+    int cur;                        // which X is the old one
+    int scaled;                     // X is still u times a power of two: the rest of the normalisation goes in here
+    float unit, plane;              // of the operands' scales, of the result's
+};
 
 // tiles of an np x cols product; of a symmetric one the tiles that reach the diagonal or lie below it
 template <int TI, int TJ>
@@ -258,13 +262,32 @@ struct MuTile {
     static_assert(F % 4 == 0 && NB * BUF * 2 <= 160 * 1024, "LDS");
 };
 
-template <int P, int TI, int TJ>
+// Reads, fetches and products of a step one by one among each other: in a row they hold the wave up
+template <int D, int L, int M, int I = 0>
+__device__ __forceinline__ void mu_interleave() {
+    if constexpr (I < L) {
+        constexpr int d0 = I * D / L, d1 = (2 * I + 1) * D / (2 * L), d2 = (I + 1) * D / L;
+        constexpr int m0 = I * M / L, m1 = (2 * I + 1) * M / (2 * L), m2 = (I + 1) * M / L;
+        if constexpr (d1 > d0) __builtin_amdgcn_sched_group_barrier(0x100, d1 - d0, 0);
+        if constexpr (m1 > m0) __builtin_amdgcn_sched_group_barrier(0x008, m1 - m0, 0);
+        if constexpr (d2 > d1) __builtin_amdgcn_sched_group_barrier(0x100, d2 - d1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        if constexpr (m2 > m1) __builtin_amdgcn_sched_group_barrier(0x008, m2 - m1, 0);
+        mu_interleave<D, L, M, I + 1>();
+    }
+}
+
+// TR: S is given with k along its columns (X itself, in place of its transpose): skt k blocks of 32 columns.  Its fragments
+// are read from LDS transposed, groups of 16 lanes taking four rows of 16; every other octet's rows are fetched four places
+// on, so that such a group finds its 128 bytes in different banks.
+template <int P, int TI, int TJ, bool TR>
 __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtiles, const _Float16* S, int64_t ss, int stiles,
                                         int KB, int ti, int tj, f32x4 (&acc)[MuTile<P, TI, TJ>::WI][MuTile<P, TI, TJ>::WJ],
                                         _Float16* b0, _Float16* b1, _Float16* b2) {
     using C = MuTile<P, TI, TJ>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave >> 1, wj = wave & 1;
+    const int place = TR ? (((lane & 15) ^ ((lane >> 4 & 1) << 2)) + (lane & 48)) * 8 : lane * 8;
     const _Float16* src[C::L];                   // this wave's fragments of block 0; rows past the matrix: its last tile again
 #pragma unroll
     for (int l = 0; l < C::L; ++l) {
@@ -273,19 +296,27 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
             const int p = f / (TI / 16), rt = min(ti * (TI / 16) + f % (TI / 16), rtiles - 1);
             src[l] = R + p * rs + (int64_t)rt * KB * FRAG;
         } else {
-            const int g = f - C::FI, p = g / (TJ / 16), rt = min(tj * (TJ / 16) + g % (TJ / 16), stiles - 1);
-            src[l] = S + p * ss + (int64_t)rt * KB * FRAG;
+            const int g = f - C::FI, p = g / (TJ / 16), i = g % (TJ / 16);
+            if constexpr (TR) {
+                const int e = i / (TJ / 32), jb = min(tj * (TJ / 32) + i % (TJ / 32), stiles / 2 - 1);
+                src[l] = S + p * ss + ((int64_t)e * (stiles / 2) + jb) * FRAG;
+            } else src[l] = S + p * ss + (int64_t)min(tj * (TJ / 16) + i, stiles - 1) * KB * FRAG;
         }
     }
     auto fetch = [&](int kb, _Float16* buf) {
         kb = kb < KB ? kb : KB - 1;              // past the end: the last block again, so that the counts below hold
+        const int64_t rk = (int64_t)kb * FRAG, sk = TR ? rk * stiles : rk;
 #pragma unroll
         for (int l = 0; l < C::L; ++l)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[l] + (int64_t)kb * FRAG + lane * 8),
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wave * C::L + l < C::FI ? src[l] + rk + lane * 8 : src[l] + sk + place),
                                              (__attribute__((address_space(3))) void*)(buf + (wave * C::L + l) * FRAG), 16, 0, 0);
     };
     struct Frags { u32x4 r[P][C::WI], s[P][C::WJ]; };
-    auto read = [&](Frags& f, const _Float16* buf) {
+    // this lane's two places in a transposed read of the even 16 columns of a k block of X
+    const int g = lane & 15, quad = lane >> 4, par = g >> 1 & 1;
+    const int t0 = ((quad >> 1) * (TJ / 32)) * FRAG + ((quad & 1) * 8 + (g >> 2) + 16 * par) * 8 + (g & 1) * 4;
+    const int tr0 = t0 + par * 32, tr1 = t0 + (1 - par) * 32;
+    auto read = [&](Frags& f, _Float16* buf) {
         const u32x4* b = reinterpret_cast<const u32x4*>(buf) + lane;
 #pragma unroll
         for (int p = 0; p < P; ++p)
@@ -294,7 +325,17 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int j = 0; j < C::WJ; ++j) f.s[p][j] = b[(C::FI + p * (TJ / 16) + wj * C::WJ + j) * 64];
+            for (int j = 0; j < C::WJ; ++j) {
+                if constexpr (TR) {
+                    const int jt = wj * C::WJ + j;
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    _Float16* at = buf + (C::FI + p * (TJ / 16) + jt / 2) * FRAG + (jt & 1) * 256;
+                    union { s16x4 h[2]; u32x4 u; } v;
+                    v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + tr0));
+                    v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + tr1));
+                    f.s[p][j] = v.u;
+                } else f.s[p][j] = b[(C::FI + p * (TJ / 16) + wj * C::WJ + j) * 64];
+            }
     };
     auto multiply = [&](const Frags& f) {
 #pragma unroll
@@ -315,23 +356,12 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
         asm volatile("s_barrier" ::: "memory");
     };
     // multiply block k (in `cur`), read block k + 1 from `next`, fetch block k + 3 into `free`, which held block k
-    auto step = [&](int k, const Frags& cur, Frags& other, const _Float16* next, _Float16* free) {
+    auto step = [&](int k, const Frags& cur, Frags& other, _Float16* next, _Float16* free) {
         arrive();
         fetch(k + 3, free);
         read(other, next);
         multiply(cur);
-        constexpr int M = P == 2 ? 3 * C::WI * C::WJ : C::WI * C::WJ, D = P * (C::WI + C::WJ);
-        // reads and fetches go out one by one among the products: in a row they hold the wave up
-        static_assert(D == 2 * C::L, "two reads to a fetch");
-#pragma unroll
-        for (int d = 0; d < C::L; ++d) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, M / D, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, M / D, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, M % D, 0);
+        mu_interleave<P * (C::WI + (TR ? 2 : 1) * C::WJ), C::L, (P == 2 ? 3 : 1) * C::WI * C::WJ>();
     };
 #pragma unroll
     for (int i = 0; i < C::WI; ++i)
@@ -359,11 +389,11 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
 // four consecutive values along k of one row: stored as hi (and lo), and read back
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 template <int P>
-__device__ __forceinline__ void split4(const float* v, f16x4& h, f16x4& l) {
+__device__ __forceinline__ void split4(const float* v, f16x4& h, f16x4& l, float plane = PLANE) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        h[r] = (_Float16)(v[r] * PLANE);
-        l[r] = P == 2 ? (_Float16)(v[r] * PLANE - (float)h[r]) : (_Float16)0.0f;
+        h[r] = (_Float16)(v[r] * plane);
+        l[r] = P == 2 ? (_Float16)(v[r] * plane - (float)h[r]) : (_Float16)0.0f;
     }
 }
 template <int P>
@@ -415,10 +445,10 @@ __device__ __forceinline__ void mu_put(const MuArgs& a, const MuMat& t, int row,
 }
 
 template <int P, int TI, int TJ, int ST>
-__global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
+__global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
     using C = MuTile<P, TI, TJ>;
     __shared__ __attribute__((aligned(16))) _Float16 b0[C::BUF], b1[C::BUF], b2[C::BUF];
-    constexpr bool sym = ST == ST_GRAM || ST == ST_POLY;
+    constexpr bool sym = ST == ST_SYM || ST == ST_POLY;
     const int w = mu_which(a, blockIdx.x), n = mu_tiles<TI, TJ>(a.mat[w].np, sym ? a.mat[w].np : a.mat[w].mp, sym);
     // workgroups go round the eight XCDs: of every matrix each XCD gets a run of neighbouring tiles, which share operands
     // in its L2
@@ -438,20 +468,22 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
             ti = band * 8 + c % h; tj = c / h;
         }
     }
-    const int cur = it & 1, nt = t.np / 16, mt = t.mp / 16;
+    const int nt = t.np / 16, mt = t.mp / 16;
     f32x4 acc[C::WI][C::WJ];
-    if (ST == ST_GRAM) mu_tile<P, TI, TJ>(pl.X(cur), pl.xs, nt, pl.X(cur), pl.xs, nt, t.mp / 32, ti, tj, acc, b0, b1, b2);
-    else if (ST == ST_POLY) mu_tile<P, TI, TJ>(pl.A, pl.as, nt, pl.A, pl.as, nt, t.np / 32, ti, tj, acc, b0, b1, b2);
-    else mu_tile<P, TI, TJ>(pl.B, pl.as, nt, pl.XT(cur), pl.xs, mt, t.np / 32, ti, tj, acc, b0, b1, b2);
+    if constexpr (sym) {
+        const bool gram = ST == ST_SYM && g.r < 0;                        // X X^T: k runs along m
+        const _Float16 *R = gram ? pl.X(g.cur) : pl.N(g.r), *S = gram ? pl.X(g.cur) : pl.N(g.s);
+        const int64_t ps = gram ? pl.xs : pl.as;
+        mu_tile<P, TI, TJ, false>(R, ps, nt, S, ps, nt, (gram ? t.mp : t.np) / 32, ti, tj, acc, b0, b1, b2);
+    } else mu_tile<P, TI, TJ, true>(pl.N(g.r), pl.as, nt, pl.X(g.cur), pl.xs, mt, t.np / 32, ti, tj, acc, b0, b1, b2);
 
     // Lane (quad, col) holds rows 4 quad .. + 3 of column col of every 16 x 16 tile.  The results go through LDS and leave it
-    // in short loops: as they lie they are four neighbours along k of the transposed plane (half a fragment by the wave),
-    // and read eight along a row, two tiles at a time, whole fragments of the plane the other way round.  (Unrolled from the
-    // registers this was 20 to 60 KB of code that every tile runs once, waiting for instructions: 25 to 44 us a tile.)
+    // in short loops: read eight along a row, two tiles at a time, they are whole fragments; as they lie they are four
+    // neighbours along k of the mirrored place (half a fragment by the wave), which symmetric results need too.
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, col = lane & 15;
     float s = 1.0f;
-    if (it == 0 && ST != ST_POLY) { double up; mu_scale(t, a.eps, up, s); }
-    const float unit = UNPLANE * UNPLANE * (ST == ST_GRAM ? s * s : s);
+    if (g.scaled) { double up; mu_scale(t, a.eps, up, s); }
+    const float unit = g.unit * (sym ? s * s : s);
     const int lane4 = (col + 16 * (quad >> 1)) * 8 + (quad & 1) * 4;     // this lane's place in a half fragment
     const int i0 = ti * (TI / 16) + (wave >> 1) * C::WI, j0 = tj * (TJ / 16) + (wave & 1) * C::WJ;
     // the A that c A^2 is added to: all of this wave's loads at once, as nothing else hides them
@@ -462,7 +494,7 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
 #pragma unroll
             for (int j = 0; j < C::WJ; ++j) {
                 const int i16 = min(i0 + i, nt - 1), j16 = min(j0 + j, nt - 1);
-                old[i][j] = plane_load<P>(pl.A + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4, pl.as);
+                old[i][j] = plane_load<P>(pl.N(g.r) + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4, pl.as);
             }
     __syncthreads();                                                     // the operands in LDS are done with
     // a wave's own 16 x 16 tiles, QI rows of them at a time; 16 bytes after every 16 lanes and every tile starts 16 banks
@@ -489,7 +521,7 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
             }
         asm volatile("" ::: "memory");           // a wave's LDS accesses are served in order: only the compiler must keep it
         constexpr int N = C::QI * C::WJ, U = N >= 4 ? 4 : N;             // U tiles' LDS reads under way at once
-        if (ST != ST_LAST || tr)
+        if (sym || (ST == ST_LAST && tr))
             for (int e0 = 0; e0 < N; e0 += U) {
                 f32x4 v4[U];
 #pragma unroll
@@ -503,12 +535,11 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
                         if (in) mu_put(a, t, j16 * 16 + col, i16 * 16 + 4 * quad, v, vec);
                     } else {
                         f16x4 h, l;
-                        split4<P>(v, h, l);
-                        _Float16* out = (sym ? (ST == ST_GRAM ? pl.A : pl.B) : pl.XT(cur ^ 1))
-                                        + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4;
+                        split4<P>(v, h, l, g.plane);
+                        _Float16* out = pl.N(g.out) + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4;
                         if (in) {
                             *reinterpret_cast<f16x4*>(out) = h;
-                            if (P == 2) *reinterpret_cast<f16x4*>(out + (sym ? pl.as : pl.xs)) = l;
+                            if (P == 2) *reinterpret_cast<f16x4*>(out + pl.as) = l;
                         }
                     }
                 }
@@ -534,14 +565,14 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, int it) {
                             mu_put(a, t, i16 * 16 + row, jp * 16 + oct * 8 + 4, v[u] + 4, vec);
                         }
                     } else {
+                        const float plane = sym ? g.plane : PLANE;
                         f16x8 h, l;
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            h[k] = (_Float16)(v[u][k] * PLANE);
-                            l[k] = (_Float16)(v[u][k] * PLANE - (float)h[k]);
+                            h[k] = (_Float16)(v[u][k] * plane);
+                            l[k] = (_Float16)(v[u][k] * plane - (float)h[k]);
                         }
-                        _Float16* out = (sym ? (ST == ST_GRAM ? pl.A : pl.B) : pl.X(cur ^ 1))
-                                        + ((int64_t)i16 * ((sym ? t.np : t.mp) >> 5) + (jp >> 1)) * FRAG + lane * 8;
+                        _Float16* out = (sym ? pl.N(g.out) : pl.X(g.cur ^ 1)) + ((int64_t)i16 * ((sym ? t.np : t.mp) >> 5) + (jp >> 1)) * FRAG + lane * 8;
                         if (in && (!sym || jp + (lane >> 5) < i16)) {    // on the diagonal the loop above stored the whole tile
                             *reinterpret_cast<f16x8*>(out) = h;
                             if (P == 2) *reinterpret_cast<f16x8*>(out + (sym ? pl.as : pl.xs)) = l;
@@ -681,10 +712,10 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
         asm volatile("" : "+v"(lane));           // addresses are made anew: kept over the steps they spill
         const float sc = it == 0 ? s : 1.0f;
 #pragma unroll 1
-        for (int st = ST_GRAM; st <= ST_POLY; ++st) {     // A = X X^T, then B = a + b A + c A^2 over it
-            const _Float16* src = st == ST_GRAM ? X : A;
-            const int64_t ps = st == ST_GRAM ? xs : as;
-            const int K = st == ST_GRAM ? mb : nb;
+        for (int st = ST_SYM; st <= ST_POLY; ++st) {     // A = X X^T, then B = a + b A + c A^2 over it
+            const _Float16* src = st == ST_SYM ? X : A;
+            const int64_t ps = st == ST_SYM ? xs : as;
+            const int K = st == ST_SYM ? mb : nb;
             f32x4 acc[MuSmall<P>::SYM][2][2];
 #pragma unroll
             for (int q = 0; q < MuSmall<P>::SYM; ++q) {
@@ -713,7 +744,7 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[0][e >> 1], o.c[0][e & 1], acc[q][e >> 1][e & 1]);
                 });
-                const float unit = UNPLANE * UNPLANE * (st == ST_GRAM ? sc * sc : 1.0f);
+                const float unit = UNPLANE * UNPLANE * (st == ST_SYM ? sc * sc : 1.0f);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i16 = 2 * bi + (e >> 1), j16 = 2 * bj + (e & 1);
@@ -821,7 +852,7 @@ constexpr int MU_PAD = 64;          // sides are padded to this; larger tiles re
 static int64_t mu_matrix_bytes(int64_t rows, int64_t cols, int P) {
     const int64_t n = rows < cols ? rows : cols, m = rows < cols ? cols : rows;
     const int64_t np = round_up(n, MU_PAD), mp = round_up(m, MU_PAD);
-    return round_up(2 * P * (4 * np * mp + 2 * np * np), 256) + MU_PARTS * 8;
+    return round_up(2 * P * (2 * np * mp + 4 * np * np), 256) + MU_PARTS * 8;
 }
 static int64_t mu_group_bytes(const mctsq_muon_matrix* mats, int count, int P) {
     int64_t o = 0;
@@ -861,9 +892,11 @@ static double mu_stage(MuArgs& a, bool sym, bool gram, double step, double over,
     const int load = (tiles + 255) / 256;
     return work / tiles * step * load + over * ((load + share - 1) / share);
 }
+// launches the stage (st != NULL-stream semantics aside), or only estimates it
 template <int P, int ST>
-static void mu_product(MuArgs& a, int it, hipStream_t st) {
-    constexpr bool sym = ST == ST_GRAM || ST == ST_POLY, gram = ST == ST_GRAM;
+static double mu_product(MuArgs& a, const MuStage& g, hipStream_t st, bool launch) {
+    constexpr bool sym = ST == ST_SYM || ST == ST_POLY;
+    const bool gram = ST == ST_SYM && g.r < 0;
     // fp32: 256 x 128 tiles 0.87 us a k block (0.73 at the matrix pipe's rate) and 23 a tile, 128 x 128 0.50 and 15, 64 x 64
     // 0.20 and 8 with three to a CU; bf16: 0.33 / 15, 0.19 / 8, 0.10 / 5
     static constexpr double STEP[2][3] = {{0.33, 0.19, 0.10}, {0.87, 0.50, 0.20}}, OVER[2][3] = {{15, 8, 5}, {23, 15, 8}};
@@ -871,16 +904,47 @@ static void mu_product(MuArgs& a, int it, hipStream_t st) {
     const double t256 = mu_stage<256, 128>(a, sym, gram, STEP[P - 1][0], OVER[P - 1][0], 1, tiles);
     const double t128 = mu_stage<128, 128>(a, sym, gram, STEP[P - 1][1], OVER[P - 1][1], P == 2 ? 1 : 2, tiles);
     const double t64 = mu_stage<64, 64>(a, sym, gram, STEP[P - 1][2], OVER[P - 1][2], 3, tiles);      // a.first as for 64 x 64
-    if (t64 <= t128 && t64 <= t256) {
-        hipLaunchKernelGGL((mu_product_kernel<P, 64, 64, ST>), dim3(tiles), dim3(256), 0, st, a, it);
-    } else if (t128 <= t256) {
+    const double best = std::min(t64, std::min(t128, t256));
+    if (!launch) return best;
+    if (t64 == best) {
+        hipLaunchKernelGGL((mu_product_kernel<P, 64, 64, ST>), dim3(tiles), dim3(256), 0, st, a, g);
+    } else if (t128 == best) {
         mu_stage<128, 128>(a, sym, gram, 0, 0, 1, tiles);
-        hipLaunchKernelGGL((mu_product_kernel<P, 128, 128, ST>), dim3(tiles), dim3(256), 0, st, a, it);
+        hipLaunchKernelGGL((mu_product_kernel<P, 128, 128, ST>), dim3(tiles), dim3(256), 0, st, a, g);
     } else {
         mu_stage<256, 128>(a, sym, gram, 0, 0, 1, tiles);
-        hipLaunchKernelGGL((mu_product_kernel<P, 256, 128, ST>), dim3(tiles), dim3(256), 0, st, a, it);
+        hipLaunchKernelGGL((mu_product_kernel<P, 256, 128, ST>), dim3(tiles), dim3(256), 0, st, a, g);
     }
+    return best;
 }
+
+// `chain` steps at once, from X_cur to the other X (or the caller's matrix).  The A of a step is a polynomial of the A of the
+// step before it, A' = Q A Q with Q = a + b A + c A^2, as X' = Q X; so the chain needs X only at its ends:
+//   A = X X^T;  per step Q = a + b A + c A^2, N <- Q N, A <- (Q A) Q;  X <- N X
+// 3 n^2 m + (4 chain - 3) n^3 in place of chain (3 n^2 m + n^3).  N's values reach 3.4445^chain, its planes 2^(16 - 2 chain).
+template <int P>
+static double mu_steps(MuArgs& a, int chain, int cur, bool scaled, bool last, hipStream_t st, bool launch) {
+    const float u2 = UNPLANE * UNPLANE;
+    // n x n matrices: 0 A, 1 .. 3 Q, N and Q A in turn
+    double t = mu_product<P, ST_SYM>(a, MuStage{-1, -1, 0, cur, scaled, u2, PLANE}, st, launch);
+    int q = 1, n = 1;
+    float np = PLANE;
+    t += mu_product<P, ST_POLY>(a, MuStage{0, 0, q, cur, 0, u2, PLANE}, st, launch);
+    for (int k = 1; k < chain; ++k) {
+        const int w = 6 - q - n == 4 ? 2 : 6 - q - n;                        // the one that is neither (any of two where q = n)
+        t += mu_product<P, ST_SYM>(a, MuStage{q, 0, w, cur, 0, u2, PLANE}, st, launch);             // Q A
+        t += mu_product<P, ST_SYM>(a, MuStage{w, q, 0, cur, 0, u2, PLANE}, st, launch);             // (Q A) Q
+        q = w;
+        t += mu_product<P, ST_POLY>(a, MuStage{0, 0, q, cur, 0, u2, PLANE}, st, launch);
+        const int o = 6 - q - n;
+        t += mu_product<P, ST_SYM>(a, MuStage{q, n, o, cur, 0, UNPLANE / np, np / 4}, st, launch);  // N
+        n = o;
+        np /= 4;
+    }
+    const MuStage end{n, -1, -1, cur, scaled, UNPLANE / np, PLANE};
+    return t + (last ? mu_product<P, ST_LAST>(a, end, st, launch) : mu_product<P, ST_NEXT>(a, end, st, launch));
+}
+
 template <int P>
 static void mu_launch(MuArgs& a, hipStream_t st) {
     bool small = true;
@@ -896,12 +960,16 @@ static void mu_launch(MuArgs& a, hipStream_t st) {
         if (i < a.count) blk += (a.mat[i].np / 64) * (a.mat[i].mp / 64);
     }
     hipLaunchKernelGGL(mu_planes_kernel<P>, dim3(blk), dim3(256), 0, st, a);
-    for (int it = 0; it < 5; ++it) {
-        mu_product<P, ST_GRAM>(a, it, st);
-        mu_product<P, ST_POLY>(a, it, st);
-        if (it < 4) mu_product<P, ST_NEXT>(a, it, st);
-        else mu_product<P, ST_LAST>(a, it, st);
-    }
+    // One step at a time, or two and then three at once where the products that saves are worth more than the launches it
+    // adds (wide and large matrices).  Errors against 64 bits are the same: 1.9e-6 one by one, 2.0e-6 two and three, 2.7e-6
+    // three and two, for 512 x 2048.
+    const double one = 5 * mu_steps<P>(a, 1, 0, false, false, st, false);
+    const double two = mu_steps<P>(a, 2, 0, false, false, st, false) + mu_steps<P>(a, 3, 0, false, false, st, false);
+    if (two < 0.95 * one) {
+        mu_steps<P>(a, 2, 0, true, false, st, true);
+        mu_steps<P>(a, 3, 1, false, true, st, true);
+    } else
+        for (int it = 0; it < 5; ++it) mu_steps<P>(a, 1, it & 1, it == 0, it == 4, st, true);
 }
 
 static int mu_run(const mctsq_muon_matrix* mats, int64_t count, int P, MuArgs& a, double lr, int adjust, char* ws, hipStream_t st) {
