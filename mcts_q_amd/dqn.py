@@ -359,7 +359,11 @@ class DQNModel:
                  embed_dim: int, hidden_layers: int, hidden_units: int, buffer_capacity: int, batch_size: int,
                  gamma: float, lr: float, price_encoder_type: str = "conv", process_encoder_type: str = "gru",
                  gas_eua_encoder_type: str = "mlp", activation: str = "relu", learning_starts: int = 10000,
-                 seed: int | None = None, device="cuda:0", seq_lens=(25, 10, 3), process_group=None):
+                 seed: int | None = None, device="cuda:0", seq_lens=(25, 10, 3), process_group=None,
+                 optimizer: str = "adam"):
+        """optimizer: "adam" (the reference's), or "muon" for the hidden weight matrices (DeviceLearner)."""
+        if optimizer == "muon" and process_group is not None:
+            raise MctsqError("optimizer='muon': update() has no data-parallel form")
         if seed is not None:                              # dqn_per.py:368-373
             torch.manual_seed(seed)
             np.random.seed(seed)
@@ -374,7 +378,7 @@ class DQNModel:
         self.policy_net = self._net_cls(*args, device=device, seq_lens=seq_lens)
         self.policy_net._check_replay_geometry(training=True)
         self.learner = DeviceLearner(self.policy_net.spec, device, gamma=gamma, lr=lr, process_group=process_group,
-                                     policy=self.policy_net.qnet)
+                                     policy=self.policy_net.qnet, optimizer=optimizer)
         # the reference constructs (and default-initialises) the target net before overwriting it
         # with the policy weights (:389-396): consume the same RNG stream
         _default_init_state_dict(el_input_dim, process_input_dim, gas_eua_input_dim, int(embed_dim),

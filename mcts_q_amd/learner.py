@@ -12,6 +12,7 @@ import ctypes as C
 import torch
 
 from ._lib import lib, ptr, stream_ptr, MctsqError, StepArgs
+from .muon import DeviceMuon
 from .netdesc import NetSpec
 from .parallel import all_reduce
 from .qnet import DeviceQNet
@@ -19,7 +20,12 @@ from .qnet import DeviceQNet
 
 class DeviceLearner:
     def __init__(self, spec: NetSpec, device="cuda:0", gamma=0.99, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
-                 max_grad_norm=10.0, process_group=None, policy: DeviceQNet | None = None):
+                 max_grad_norm=10.0, process_group=None, policy: DeviceQNet | None = None, optimizer: str = "adam",
+                 muon_lr=0.02, muon_momentum=0.95):
+        """optimizer "muon": hidden weight matrices (`muon_keys()`) move by DeviceMuon steps of rate `muon_lr` on the
+        unclipped gradient, their momentum in exp_avg; everything else by the clipped Adam step of rate `lr`."""
+        if optimizer not in ("adam", "muon"):
+            raise ValueError(f"optimizer: expected 'adam' or 'muon', got {optimizer!r}")
         if not torch.cuda.is_available():
             raise MctsqError("DeviceLearner needs a GPU: the HIP path has no CPU fallback")
         self.spec, self.device = spec, torch.device(device)
@@ -55,6 +61,31 @@ class DeviceLearner:
         nparts = lib.check(lib.mctsq_dqn_grad_sumsq_parts(C.byref(self.desc)))
         self._sumsq_parts = torch.zeros(nparts, dtype=torch.float64, device=self.device)
         self._n_sumsq = C.c_int64(0)
+        self.optimizer = optimizer
+        if optimizer == "muon":
+            keys = self.muon_keys()
+            views, grads = self.policy.views(), self.policy.views(self.grad)
+            mom = self.policy.views(self.exp_avg)
+            self.muon = DeviceMuon([views[k] for k in keys], lr=muon_lr, momentum=muon_momentum,
+                                   momentum_buffers=[mom[k] for k in keys])
+            self._muon_grads = [grads[k] for k in keys]
+            # what is left for Adam: runs of the flat buffer between those matrices (tensor starts are padded to 16 floats)
+            offs, _, total = spec.layout()
+            runs, at = [], 0
+            for (k, _), o, e in zip(spec.param_keys(), offs, list(offs[1:]) + [total]):
+                if k in keys:
+                    if o > at:
+                        runs.append((int(at), int(o)))
+                    at = e
+            if total > at:
+                runs.append((int(at), int(total)))
+            self._adam_runs = runs
+
+    def muon_keys(self):
+        """The weights a Muon step is made for: matrices between hidden layers, both sides at least 16, without the layer
+        that gives the action values."""
+        last = f"fc_layers.{2 * self.spec.hidden_layers}.weight"
+        return [k for k, s in self.spec.param_keys() if len(s) == 2 and min(s) >= 16 and k != last and "pos" not in k]
 
     def _st(self):
         return stream_ptr(self.device)
@@ -134,6 +165,9 @@ class DeviceLearner:
         """tau None: no target update in this call; 0 < tau <= 1: Polyak (1.0 = hard copy)."""
         self.step_count += 1
         n = self.spec.n_flat
+        if self.optimizer == "muon":
+            self._apply_muon(tau)
+            return
         parts = getattr(self, "_have_sumsq", False)
         lib.check(lib.mctsq_clip_adam_polyak_ex(
             ptr(self.policy.flat), ptr(self.grad), ptr(self.exp_avg), ptr(self.exp_avg_sq),
@@ -143,6 +177,25 @@ class DeviceLearner:
             ptr(self._small), self._small.numel(), self._st()))
         self._have_sumsq = False                # the pieces describe one gradient, used once
         self._prepare()                         # policy (and target) changed: one launch refreshes every fragment
+
+    def _apply_muon(self, tau):
+        """DeviceMuon on its matrices, clip + Adam with the norm of the WHOLE gradient on the runs between them, then the
+        target."""
+        if getattr(self, "_have_sumsq", False):
+            sumsq, nparts = self._sumsq_parts, self._n_sumsq.value
+        else:
+            sumsq, nparts = torch.linalg.vector_norm(self.grad, dtype=torch.float64).square().reshape(1), 1
+        self.muon.step(self._muon_grads)
+        for a, b in self._adam_runs:
+            lib.check(lib.mctsq_clip_adam_polyak_ex(
+                ptr(self.policy.flat[a:b]), ptr(self.grad[a:b]), ptr(self.exp_avg[a:b]), ptr(self.exp_avg_sq[a:b]), None,
+                b - a, self.step_count, self.lr, self.betas[0], self.betas[1], self.eps, self.max_grad_norm, -1.0,
+                ptr(self.grad_norm), ptr(sumsq), nparts, ptr(self._small), self._small.numel(), self._st()))
+        if tau is not None:
+            lib.check(lib.mctsq_polyak(ptr(self.policy.flat), ptr(self.target.flat), self.spec.n_flat, float(tau),
+                                       self._st()))
+        self._have_sumsq = False
+        self._prepare()
 
     # ---- DQNModel.update() as ONE library call (dqn_per.py:401-476) ---------------------------------
     def step(self, replay, u, tau: float | None = None, beta: float = 0.4):
@@ -156,6 +209,12 @@ class DeviceLearner:
             raise ValueError("cannot sample from an empty buffer")
         u = torch.as_tensor(u, dtype=torch.float64).to(self.device).contiguous()
         B = int(u.numel())
+        if self.optimizer == "muon":            # the one-call step is Adam's: the separate entry points
+            batch, isw, idx, _ = replay.sample_batch(u, beta)
+            abs_td = self.compute_grad(batch, isw)
+            self.apply_grad(tau)
+            replay.update_priorities(idx, abs_td)
+            return
         # Deferred re-split: the call re-splits the weight fragments at its START, on a helper lane under the sampling
         # launch, and leaves them stale at its end (one launch and one boundary less on the step's serial chain).
         # Whoever needs the fragments next re-splits them itself: the next step(), compute_grad() through
@@ -200,6 +259,9 @@ class DeviceLearner:
         over [gradient | loss | weight-maximum slots]; nothing is read back to the host (the (kept, dropped) counters
         of a step are looked at one step later).  Works at world == 1 too (same results as step() up to the fp32
         rounding of the weight division, include/mctsq_hip.h)."""
+        if self.optimizer == "muon":
+            raise MctsqError("the two-call data-parallel step is Adam's; with optimizer='muon' use compute_grad / "
+                             "apply_grad (parallel.ShardedSampler)")
         from .parallel import all_gather_rows, draw_capacity
         u = torch.as_tensor(u, dtype=torch.float64).to(self.device).contiguous()
         B = int(u.numel())
