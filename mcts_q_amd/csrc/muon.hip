@@ -960,16 +960,24 @@ static void mu_launch(MuArgs& a, hipStream_t st) {
         if (i < a.count) blk += (a.mat[i].np / 64) * (a.mat[i].mp / 64);
     }
     hipLaunchKernelGGL(mu_planes_kernel<P>, dim3(blk), dim3(256), 0, st, a);
-    // One step at a time, or two and then three at once where the products that saves are worth more than the launches it
-    // adds (wide and large matrices).  Errors against 64 bits are the same: 1.9e-6 one by one, 2.0e-6 two and three, 2.7e-6
-    // three and two, for 512 x 2048.
-    const double one = 5 * mu_steps<P>(a, 1, 0, false, false, st, false);
-    const double two = mu_steps<P>(a, 2, 0, false, false, st, false) + mu_steps<P>(a, 3, 0, false, false, st, false);
-    if (two < 0.95 * one) {
-        mu_steps<P>(a, 2, 0, true, false, st, true);
-        mu_steps<P>(a, 3, 1, false, true, st, true);
-    } else
-        for (int it = 0; it < 5; ++it) mu_steps<P>(a, 1, it & 1, it == 0, it == 4, st, true);
+    // One step at a time; or two, one, two at once, or two and three, where the products that saves are worth more than the
+    // launches it adds (large matrices, the wider the more).  Errors against 64 bits, fp32, worst of five shapes and three
+    // spectra (elementary fp32 operations 5.6e-6 and 1.3e-4 where four directions carry all but 1e-3): one by one 3.6e-6
+    // and 1.5e-4, two-one-two 3.1e-6 and 9.5e-5, two-three 4.4e-6 and 9.8e-5, the 4.4e-6 at 1000 x 1500, hence 2 n <= m.
+    // bf16 (rounding alone 1.7e-3): 2.2e-3 and 3.9e-2, 2.2e-3 and 9.9e-3, 4.2e-3 and 6.1e-2: never two-three.
+    static constexpr int PLAN[3][6] = {{1, 1, 1, 1, 1, 0}, {2, 1, 2, 0, 0, 0}, {2, 3, 0, 0, 0, 0}};
+    double one = 0.0, cost[4];
+    for (int c = 1; c <= 3; ++c) cost[c] = mu_steps<P>(a, c, 0, false, false, st, false);
+    bool wide = P == 2;
+    for (int i = 0; i < a.count; ++i) wide = wide && a.mat[i].m >= 2 * a.mat[i].n;
+    int plan = 0;
+    for (int i = 0; i < (wide ? 3 : 2); ++i) {
+        double t = i == 0 ? 0.0 : 5.0;                                       // us of launches
+        for (int c = 0; PLAN[i][c]; ++c) t += cost[PLAN[i][c]];
+        if (i == 0 || t < 0.97 * one) { one = t; plan = i; }
+    }
+    for (int c = 0, cur = 0; PLAN[plan][c]; ++c, cur ^= 1)
+        mu_steps<P>(a, PLAN[plan][c], cur, c == 0, PLAN[plan][c + 1] == 0, st, true);
 }
 
 static int mu_run(const mctsq_muon_matrix* mats, int64_t count, int P, MuArgs& a, double lr, int adjust, char* ws, hipStream_t st) {

@@ -39,6 +39,16 @@ def _slices(t):
     return [t.data_ptr() + i * step for i in range(t.shape[0])]
 
 
+def _span(t):
+    """[first, last) byte addresses a strided tensor touches."""
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())))
+
+
+def _rows_overlap(t):
+    """Whether the rows of a stack share memory with each other."""
+    return t.dim() == 3 and t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * _ld(t) + t.shape[2]
+
+
 def orthogonalize(x, eps=1e-7, out=None):
     """The iteration on `x` [rows, cols] or each matrix of [count, rows, cols], fp32 or bf16, rows contiguous.  Returns a
     tensor of the same shape and type (`out` if given; `out` may be `x`)."""
@@ -51,9 +61,12 @@ def orthogonalize(x, eps=1e-7, out=None):
                          f"with strides {x.stride()}")
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not _is_matrix(out) \
-            or (out.dim() == 3 and out.shape[0] > 1 and out.stride(0) < (out.shape[1] - 1) * _ld(out) + out.shape[2]):
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not _is_matrix(out) or _rows_overlap(out):
         raise ValueError(f"out: expected {tuple(x.shape)} {x.dtype} on {x.device} with contiguous rows that do not overlap")
+    elif not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+        (a0, a1), (b0, b1) = _span(x), _span(out)
+        if a0 < b1 and b0 < a1:
+            raise ValueError("out: must be x itself or share no memory with it")
     r, c = x.shape[-2:]
     src, dst = _slices(x), _slices(out)
     lx, lo = _ld(x), _ld(out)
@@ -85,10 +98,15 @@ class DeviceMuon:
         for i, p in enumerate(params):
             if not isinstance(p, torch.Tensor) or not p.is_cuda:
                 raise MctsqError("DeviceMuon needs parameters on the GPU: the HIP path has no CPU fallback")
-            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != params[0].device \
-                    or (p.dim() == 3 and p.shape[0] > 1 and p.stride(0) < (p.shape[1] - 1) * _ld(p) + p.shape[2]):
+            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != params[0].device or _rows_overlap(p):
                 raise ValueError(f"params[{i}]: expected fp32 [rows, cols] or [count, rows, cols] with contiguous rows on "
                                  f"{params[0].device}, got {tuple(p.shape)} {p.dtype} with strides {p.stride()} on {p.device}")
+        spans = sorted((*_span(p), i) for i, p in enumerate(params) if p.is_contiguous())
+        for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
+            if start < end:
+                raise ValueError(f"params[{i}] and params[{j}] share memory")
+        if len({p.data_ptr() for p in params}) < len(params):
+            raise ValueError("params: the same matrix twice")
         if adjust not in _ADJUST:
             raise ValueError(f"adjust: expected one of {sorted(_ADJUST)}, got {adjust!r}")
         if not 0.0 <= momentum < 1.0:
@@ -111,6 +129,7 @@ class DeviceMuon:
         with on_device(self.device):
             self._ws_bytes = lib.check(lib.mctsq_muon_workspace_bytes(self._mats, len(mats)))
             self._ws = _aligned(self._ws_bytes, self.device)
+            self._ws_stream = stream_ptr(self.device)
 
     def step(self, grads, lr=None):
         """One update from `grads` (a sequence in the order of the parameters)."""
@@ -127,6 +146,8 @@ class DeviceMuon:
             for j, q in enumerate(_slices(g)):
                 self._mats[at + j].d_x, self._mats[at + j].ldx = q, ld
         with on_device(self.device):
+            if stream_ptr(self.device) != self._ws_stream and not torch.cuda.is_current_stream_capturing():
+                self._ws.record_stream(torch.cuda.current_stream(self.device))       # not reused before that work is done
             lib.check(lib.mctsq_muon_step(self._mats, len(self._mats), _DTYPE[dt], self.lr if lr is None else float(lr),
                                           self.momentum, int(self.nesterov), self.weight_decay, self.eps,
                                           _ADJUST[self.adjust], ptr(self._ws), self._ws_bytes, stream_ptr(self.device)))

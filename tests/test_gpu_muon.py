@@ -67,6 +67,34 @@ def test_large_tiles_and_many_matrices(dtype):
     _close(orthogonalize(z), _truth(z), TOL[dtype])
 
 
+@pytest.mark.parametrize("shape,dtype", [((1, 1024, 4096), torch.float32), ((1, 2300, 1024), torch.bfloat16),
+                                         ((8, 1024, 1000), torch.float32), ((6, 1024, 1024), torch.bfloat16),
+                                         ((1, 577, 4100), torch.float32), ((2, 3000, 513), torch.float32)],
+                         ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v)[6:])
+def test_every_plan_and_tile(shape, dtype):
+    """Sizes at which several steps are made at once on the smaller side, and the largest tiles, with ragged ends."""
+    from mcts_q_amd.muon import orthogonalize
+    x = _rand(shape, sum(shape), dtype)
+    _close(orthogonalize(x), _truth(x), TOL[dtype])
+
+
+def test_a_mixed_list_of_large_and_small():
+    """One step of 23 matrices (more than one launch group) from 8 x 9 to 1500 x 600, a NaN in one of them."""
+    from mcts_q_amd.muon import DeviceMuon
+    shapes = [(8, 9), (1500, 600), (600, 1500), (64, 64), (700, 700)] + [(32 + i, 100) for i in range(18)]
+    params = [_rand(s, i) for i, s in enumerate(shapes)]
+    start = [p.double() for p in params]
+    grads = [_rand(s, 50 + i) for i, s in enumerate(shapes)]
+    grads[3][5, 5] = float("nan")
+    DeviceMuon(params, lr=0.1, momentum=0.5, adjust="none").step(grads)
+    for i, (p, s, g) in enumerate(zip(params, start, grads)):
+        if i == 3:
+            assert p.isnan().all()
+            continue
+        want = s - 0.1 * _truth(g.double() * 1.5)
+        assert (p.double() - want).norm() <= TOL[torch.float32] * (want - s).norm() + 2.0 ** -23 * want.norm(), i
+
+
 def test_known_results():
     """Rank one: the iteration acts on the one singular value, 1.  Zero: zero.  1 x 1: the sign times the same value."""
     from mcts_q_amd.muon import orthogonalize
@@ -214,7 +242,8 @@ def test_state_and_refusals():
                 lambda: orthogonalize(z[:0]), lambda: orthogonalize(z, out=z[:3]), lambda: orthogonalize(z, out=z.bfloat16()),
                 lambda: DeviceMuon([z.bfloat16()]), lambda: DeviceMuon([z.t()]), lambda: DeviceMuon([z], adjust="x"),
                 lambda: DeviceMuon([z], momentum=1.0), lambda: DeviceMuon([z], momentum_buffers=[z[:3]]),
-                lambda: DeviceMuon([z[:1].expand(6, 8)]), lambda: opt.step(g[:1]), lambda: opt.step([g[0], g[1].bfloat16()]),
+                lambda: DeviceMuon([z[:1].expand(6, 8)]), lambda: DeviceMuon([z, z]), lambda: DeviceMuon([z, z.view(12, 4)]),
+                lambda: DeviceMuon([z.view(2, 3, 8), z[3:]]), lambda: orthogonalize(z[:, :4], out=z[:, 2:6]), lambda: opt.step(g[:1]), lambda: opt.step([g[0], g[1].bfloat16()]),
                 lambda: opt.step([g[0].t(), g[1]]), lambda: opt.step([g[0].half(), g[1].half()]),
                 lambda: opt.load_state_dict({"momentum_buffers": [z, z]})):
         with pytest.raises(ValueError):
