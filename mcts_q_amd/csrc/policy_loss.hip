@@ -9,7 +9,7 @@
 //     lane, every lane with a running (max, sum of exponentials); the pairs are joined over the waves with one barrier, one
 //     thread turns them into the coefficient.  Where U vectors a lane hold the whole row (HOLD), the exponentials stay in
 //     registers and the gradient is one product per element; longer rows are read a second time, now from the caches.
-//   - rows of at most 256 elements go to groups of 4 or 16 lanes and stay in registers, many rows to a workgroup.
+//   - rows of at most 256 elements go to groups of 1, 4 or 16 lanes and stay in registers, many rows to a workgroup.
 // Statistics: exponentials and the sums of one lane in fp32 (at most 32 terms between two rescalings), everything joined
 // across lanes, the logarithm, ratio, KL term and loss in fp64: the clip decides on a ratio that two evaluations must agree
 // on.  Rows of weight 0 are padding: their logits, action, and statistics are not read, their outputs are exactly 0.
@@ -193,14 +193,15 @@ __device__ __forceinline__ double rescaled(float m, double s, float M) {
     const double r = s * (double)exp_diff_sum(m, finite_or_zero(M));
     return m > -INFINITY || s != s ? r : 0.0;            // an empty set, or one of -inf only; NaN stays
 }
-// join over groups of W = 4, 16 or 64 consecutive lanes: every lane gets the group's max and sum
+// join over groups of W = 1, 4, 16 or 64 consecutive lanes: every lane gets the group's max and sum
 template <int W>
 __device__ __forceinline__ void join_lanes(float& m, double& s) {
+    if constexpr (W == 1) return;
     float M = m;
     if constexpr (W == 4) {
         M = fmaxf(M, dpp_row<0xB1>(M));                  // quad_perm [1,0,3,2], [2,3,0,1]
         M = fmaxf(M, dpp_row<0x4E>(M));
-    } else M = row16_max_dpp(M);
+    } else if constexpr (W > 1) M = row16_max_dpp(M);
     if constexpr (W == 64) M = fmaxf(fmaxf(lane_f32(M, 0), lane_f32(M, 16)), fmaxf(lane_f32(M, 32), lane_f32(M, 48)));
     s = rescaled(m, s, M);
     if constexpr (W == 4) {
@@ -508,7 +509,9 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
         float x[EPL], m = -INFINITY, lane_m = 0.0f, inv, coef = 0.0f, za = 0.0f, s = 0.0f;
 #pragma unroll
         for (int k = 0; k < EPL; ++k) {
-            x[k] = live && g + k * G < a.V ? Elem<T>::load(z, g + k * G) : -INFINITY;
+            x[k] = -INFINITY;
+            if (k * G >= a.V) continue;                                   // the whole launch agrees
+            if (live && g + k * G < a.V) x[k] = Elem<T>::load(z, g + k * G);
             m = fmaxf(m, x[k]);
         }
         if constexpr (MODE != MODE_GRAD) {
@@ -516,7 +519,8 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
             const float ref = finite_or_zero(m);
             lane_m = m;
 #pragma unroll
-            for (int k = 0; k < EPL; ++k) s += x[k] = exp_diff_sum(x[k], ref);
+            for (int k = 0; k < EPL; ++k)
+                if (k * G < a.V) s += x[k] = exp_diff_sum(x[k], ref);
             double sd = (double)s;
             join_lanes<G>(m, sd);
             inv = fast_rcp((float)sd);
@@ -527,7 +531,7 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
                     if (bad) loss = NAN;
                 }
             }
-            if constexpr (MODE == MODE_POLICY) coef = __shfl(coef, (threadIdx.x & 63) & ~(G - 1), 64);
+            if constexpr (MODE == MODE_POLICY && G > 1) coef = __shfl(coef, (threadIdx.x & 63) & ~(G - 1), 64);
         } else {
             m = live ? a.stat_m[row] : 0.0f; inv = live ? a.stat_inv[row] : 0.0f;
             coef = live ? w * a.seq_coef[row_group(a, row)] : 0.0f;
@@ -566,61 +570,66 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const double* __restrict
     if (threadIdx.x == 0) *loss = (float)acc;
 }
 
-// One wave per pair: the two sequences' weighted sums of log-probabilities, the margin
+// A workgroup takes 64 pairs: its 16 waves add up the two sequences' weighted log-probabilities of four pairs each, then
+// 64 lanes evaluate a pair each: the margin
 //   h = beta ((S_c - R_c) - (S_r - R_r)),
 // the pair's loss -(1 - e) log sigmoid(h) - e log sigmoid(-h) and d loss / d S_c = -d loss / d S_r
-//   = beta scale u (e - sigmoid(-h)),  u the pair's weight.  A launch of one workgroup walks all pairs and adds the loss up.
+//   = beta scale u (e - sigmoid(-h)),  u the pair's weight.
 struct PairArgs {
     const double* logp64; const float* w; const float* ref; const float* pair_w;
     int64_t P, T;
     double beta, smooth, scale;
-    float* seq_logp; float* margin; float* seq_coef; double* pair_loss; float* loss;
+    float* seq_logp; float* margin; float* seq_coef; double* loss_part; float* loss;
 };
-constexpr int PAIR_WAVES = 16;
-__global__ __launch_bounds__(PAIR_WAVES * 64) void pair_kernel(PairArgs a) {
-    __shared__ double red[PAIR_WAVES];
-    const int lane = threadIdx.x & 63;
-    double total = 0.0;
-    for (int64_t p = (int64_t)blockIdx.x * PAIR_WAVES + (threadIdx.x >> 6); p < a.P; p += (int64_t)gridDim.x * PAIR_WAVES) {
-        double S[2];
+constexpr int PAIRS = 64;
+__global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
+    __shared__ double S[2 * PAIRS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t base = (int64_t)blockIdx.x * PAIRS;
+    double acc[8];                                                        // [pair of four][side]
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const int64_t r0 = (p + side * a.P) * a.T;
-            double acc = 0.0;
-            for (int64_t t0 = lane; t0 < a.T; t0 += 4 * 64) {             // four loads in flight, added in order
-                double v[4];
+    for (int q = 0; q < 8; ++q) acc[q] = 0.0;
+    for (int64_t t = lane; t < a.T; t += 64) {                            // eight loads under way, each sum in order
+        double v[8];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int64_t t = t0 + 64 * u;
-                    const float w = t < a.T ? (a.w ? a.w[r0 + t] : 1.0f) : 0.0f;
-                    v[u] = t < a.T ? a.logp64[r0 + t] : 0.0;
-                    v[u] = w != 0.0f ? (double)w * v[u] : 0.0;
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) acc += v[u];
-            }
-            S[side] = wave_sum_f64(acc);
+        for (int q = 0; q < 8; ++q) {
+            const int64_t p = base + wave + 16 * (q >> 1), row = (p + (q & 1) * a.P) * a.T + t;
+            const bool in = p < a.P;
+            const float w = in ? (a.w ? a.w[row] : 1.0f) : 0.0f;
+            const double l = in ? a.logp64[row] : 0.0;
+            v[q] = w != 0.0f ? (double)w * l : 0.0;
         }
-        if (lane == 0) {
-            const double h = a.beta * ((S[0] - (double)a.ref[p]) - (S[1] - (double)a.ref[p + a.P]));
-            const double t = log1p(exp(-fabs(h))), up = t + fmax(-h, 0.0), down = t + fmax(h, 0.0);
-            const double u = a.pair_w ? (double)a.pair_w[p] : 1.0, sw = a.scale * u;
-            const double dn = 1.0 / (1.0 + exp(h));                        // sigmoid(-h)
-            const bool live = u != 0.0;
-            const double c = live ? a.beta * sw * (a.smooth - dn) : 0.0;
-            a.seq_logp[p] = (float)S[0]; a.seq_logp[p + a.P] = (float)S[1];
-            a.margin[p] = live ? (float)h : 0.0f;
-            a.seq_coef[p] = (float)c; a.seq_coef[p + a.P] = (float)-c;
-            double l = sw * ((1.0 - a.smooth) * up + a.smooth * down);
-            if (h != h) l = h * sw;
-            if (!live) l = 0.0;
-            a.pair_loss[p] = l;
-            total += l;
-        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += v[q];
     }
-    if (a.loss) {
-        total = block_sum_f64(total, red);
-        if (threadIdx.x == 0) *a.loss = (float)total;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const double s = wave_sum_f64(acc[q]);
+        if (lane == 0) S[2 * (wave + 16 * (q >> 1)) + (q & 1)] = s;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    const int64_t p = base + lane;
+    double l = 0.0;
+    if (p < a.P) {
+        const double Sc = S[2 * lane], Sr = S[2 * lane + 1];
+        const double h = a.beta * ((Sc - (double)a.ref[p]) - (Sr - (double)a.ref[p + a.P]));
+        const double t = log1p(exp(-fabs(h))), up = t + fmax(-h, 0.0), down = t + fmax(h, 0.0);
+        const double u = a.pair_w ? (double)a.pair_w[p] : 1.0, sw = a.scale * u;
+        const double dn = 1.0 / (1.0 + exp(h));                            // sigmoid(-h)
+        const bool live = u != 0.0;
+        const double c = live ? a.beta * sw * (a.smooth - dn) : 0.0;
+        a.seq_logp[p] = (float)Sc; a.seq_logp[p + a.P] = (float)Sr;
+        a.margin[p] = live ? (float)h : 0.0f;
+        a.seq_coef[p] = (float)c; a.seq_coef[p + a.P] = (float)-c;
+        l = sw * ((1.0 - a.smooth) * up + a.smooth * down);
+        if (h != h) l = h * sw;
+        if (!live) l = 0.0;
+    }
+    l = wave_sum_f64(l);
+    if (lane == 0) {
+        if (gridDim.x == 1) *a.loss = (float)l;
+        else a.loss_part[blockIdx.x] = l;
     }
 }
 
@@ -637,14 +646,16 @@ static int64_t launch_rows(const RowArgs& a, hipStream_t st) {
         return grid;                                                                              \
     } while (0)
     const int64_t bytes = a.V * (int64_t)sizeof(T);
-    if (a.V <= 32) {
-        // up to 1024 rows (the agent's batch) one workgroup takes them all and adds its own loss up: one launch
+    if (a.V <= 8) {
+        // a lane per row.  Up to 1024 rows (the agent's batch of 1024 over 5 actions) one workgroup takes them all and adds
+        // its own loss up: one launch
         if (MODE == MODE_POLICY && a.rows <= 1024) {
-            hipLaunchKernelGGL((row_lane_kernel<T, 4, 8, 1024, MODE>), dim3(1), dim3(1024), 0, st, a);
+            hipLaunchKernelGGL((row_lane_kernel<T, 1, 8, 1024, MODE>), dim3(1), dim3(1024), 0, st, a);
             return 1;
         }
-        MCTSQ_ROWS(256, 64, row_lane_kernel<T, 4, 8, 256, MODE>);
+        MCTSQ_ROWS(256, 256, row_lane_kernel<T, 1, 8, 256, MODE>);
     }
+    if (a.V <= 32) MCTSQ_ROWS(256, 64, row_lane_kernel<T, 4, 8, 256, MODE>);
     if (a.V <= 256) MCTSQ_ROWS(256, 16, row_lane_kernel<T, 16, 16, 256, MODE>);
     // Measured (policy loss, 2 V bytes a bf16 row, 33 to 270 MB of logits; GB/s read + written): waves per row and vectors
     // per lane so that one row just fits keeps the most rows in flight -- V = 2040 RW 1 U 4 3900 (RW 2 2830), 8184 RW 2 U 8
@@ -728,7 +739,7 @@ static int64_t pref_ws(int64_t seqs, int64_t T, int64_t* off) {
     off[2] = take(rows * 4);            // stat_inv
     off[3] = take(rows * 4);            // logp (fp32, when the caller wants none)
     off[4] = take(seqs * 4);            // seq_coef
-    off[5] = take(seqs / 2 * 8);        // pair_loss
+    off[5] = take((seqs / 2 + PAIRS - 1) / PAIRS * 8);      // loss_part
     return o < 16 ? 16 : o;
 }
 
@@ -815,7 +826,7 @@ extern "C" int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pa
     PairArgs p{};
     p.logp64 = a.logp64; p.w = d_weight; p.ref = d_ref_logp; p.pair_w = d_pair_weight; p.P = pairs; p.T = tokens;
     p.beta = beta; p.smooth = label_smoothing; p.scale = loss_scale;
-    p.seq_logp = d_seq_logp; p.margin = d_margin; p.seq_coef = (float*)(ws + off[4]); p.pair_loss = (double*)(ws + off[5]);
+    p.seq_logp = d_seq_logp; p.margin = d_margin; p.seq_coef = (float*)(ws + off[4]); p.loss_part = (double*)(ws + off[5]); p.loss = d_loss;
     // The gradient reads the logits again, from memory where they are larger than the caches (8 pairs of 102 MB: 398 us at
     // 5.15 TB/s for two readings and one writing would be 359; pairs sent through in groups of 32 to 224 MB so that the
     // second reading could find them cached took 485 to 529).
@@ -824,13 +835,10 @@ extern "C" int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pa
         f.dz = nullptr;
         launch_rows<MODE_LOGP>(dtype, f, st);
     }
-    // up to 64 pairs one workgroup walks them and adds the loss up (four pairs to a wave); more are spread, and summed after
-    const bool one = pairs <= 64;
-    const int64_t pg = one ? 1 : (pairs + PAIR_WAVES - 1) / PAIR_WAVES;
-    p.loss = one ? d_loss : nullptr;
-    hipLaunchKernelGGL(pair_kernel, dim3((unsigned)(pg < MAX_GRID ? pg : MAX_GRID)), dim3(PAIR_WAVES * 64), 0, st, p);
+    const int64_t pg = pairs > 0 ? (pairs + PAIRS - 1) / PAIRS : 1;        // no pairs: the launch writes loss 0
+    hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pg), dim3(1024), 0, st, p);
     if (rows > 0 && d_dlogits) launch_rows<MODE_GRAD>(dtype, a, st);
-    if (!one) hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)p.pair_loss, pairs, d_loss);
+    if (pg > 1) hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, st, (const double*)p.loss_part, pg, d_loss);
     MCTSQ_HIP(hipGetLastError());
     return 0;
 }

@@ -238,7 +238,7 @@ def test_offsets_past_32_bits():
     _check_logp(token_logprobs(z, a), _logp64(z, a))
 
 
-@pytest.mark.parametrize("P,T,V,dtype", [(1, 1, 2, "fp32"), (64, 25, 5, "fp32"), (3, 1, 300, "bf16"), (2, 37, 1031, "fp16"),
+@pytest.mark.parametrize("P,T,V,dtype", [(1, 1, 2, "fp32"), (64, 25, 5, "fp32"), (65, 3, 7, "bf16"), (200, 2, 9, "fp16"), (3, 1, 300, "bf16"), (2, 37, 1031, "fp16"),
                                          (2, 5, 33001, "bf16"), (1, 300, 17, "bf16"), (2, 3, 131072, "bf16")])
 @pytest.mark.parametrize("smooth", [0.0, 0.1])
 def test_preference_loss(P, T, V, dtype, smooth):
