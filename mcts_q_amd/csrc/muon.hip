@@ -1,24 +1,28 @@
 // Orthogonalised updates: momentum, five quintic Newton-Schulz steps on each weight matrix, decay and update.
 //
 //   u = g + mu m' (m' = mu m + g),  X_0 = u / (|u|_F + eps),
-//   A = X X^T,  B = b A + c A^2,  X <- a X + B X        (a, b, c) = (3.4445, -4.7750, 2.0315), n = rows <= m = columns
+//   A = X X^T,  Q = a + b A + c A^2,  X <- Q X          (a, b, c) = (3.4445, -4.7750, 2.0315), n = rows <= m = columns
 //
 // which maps every singular value s of X through a s + b s^3 + c s^5, towards 1 (tall matrices are worked on transposed).
-// Per step n^2 m + n^3 + 2 n^2 m fused multiply-adds: A and B are symmetric, only tiles on and below the diagonal are
-// computed and stored to both places.  The bound is the matrix pipe.
+// Per step n^2 m + n^3 + 2 n^2 m operations: A and Q are symmetric, only tiles that reach the diagonal or lie below it are
+// computed, and stored to both places.  The bound is the matrix pipe from n = 1024 up, the chain of dependent launches below.
 //
 // Arithmetic.  fp32 matrices go through the two-way fp16 split of this library (device_utils.hpp: split2h): every operand is
 // hi + lo in fp16 scaled by 2^14, products lo hi + hi lo + hi hi accumulate in fp32, i.e. fp32 accuracy at three 16-bit
-// matrix instructions.  The scale is safe without looking at the data: |u|_F = 1 bounds every singular value of X_0 by 1,
-// the quintic maps [0, 1.21] into itself, so |X| <= 1.21, |A| <= 1.47, |B| <= 2.81 and 2.81 * 2^14 < 65504.
-// bf16 matrices use the hi plane alone: one matrix instruction per product; X, A and B are rounded to 11 bits each step,
-// which leaves the result 1.2e-3 off in the mean against 1.7e-3 for its rounding to bf16.
+// matrix instructions (a library fp32 product reaches 153 TFLOP/s on this card, the fp16 one 1220).  The scale is safe
+// without looking at the data: |u|_F = 1 bounds every singular value of X_0 by 1, the quintic maps [0, 1.21] into itself, so
+// |X| <= 1.21, |A| <= 1.47, |Q| <= 3.4445 and 3.4445 * 2^14 < 65504.
+// bf16 matrices use the hi plane alone: one matrix instruction per product; X, A and Q are rounded to 11 bits each step,
+// which leaves the result 1.9e-3 to 2.2e-3 off where its rounding to bf16 alone is 1.7e-3.  Directions weaker than 2^-11 of
+// the strongest are lost in those 11 bits (four directions carrying all but 1e-3: 1e-2 to 4e-2 off).
 // X_0 is never rounded by the normalisation: its planes hold u times a power of two, the rest of the factor (in (1, 2])
 // enters the first step's products in fp32.
 //
 // Planes are stored as the matrix instruction's operand fragments, [row tile of 16][k block of 32][lane 64][8], 1 KB in a
-// row per fragment, so a tile is fetched into LDS lane by lane (global_load_lds) and read back without a bank conflict.
-// X is kept both ways (k along m for A, k along n for B X).
+// row per fragment, so a tile is fetched into LDS lane by lane (global_load_lds) and read back without a bank conflict.  X is
+// kept one way: k along m for A; for Q X, k along n, its fragments are read from LDS transposed.
+// Measured (one layer of width 2048: four 2048 x 2048, three 8192 x 2048, a step): 5.36 ms, products at 1.1 of the 1.22
+// PFLOP/s of a large library product; 72 us for the agent's five matrices in the one-workgroup form.
 #include <limits.h>
 #include <math.h>
 
@@ -104,15 +108,24 @@ __global__ __launch_bounds__(256) void mu_norm_kernel(MuArgs a) {
             for (int c = 0; c < 4; ++c) acc = fma((double)u[c], (double)u[c], acc);
         }
     }
-    for (int64_t i = tail + tid; i < total; i += nt) {
-        const int64_t r = flat ? 0 : i / t.cols, c = i - r * t.cols;
-        float u = mu_load(t.x, r * t.ldx + c, a.xtype);
-        if (t.mom) {
-            float m = t.mom[i];
-            u = mu_update(a, u, m);
-            t.mom[i] = m;
+    for (int64_t i0 = tail + tid; i0 < total; i0 += 4 * nt) {             // four elements under way
+        float g[4], m[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = i0 + u * nt < total ? i0 + u * nt : i0, r = flat ? 0 : i / t.cols;
+            g[u] = mu_load(t.x, r * t.ldx + (i - r * t.cols), a.xtype);
+            m[u] = t.mom ? t.mom[i] : 0.0f;
         }
-        acc = fma((double)u, (double)u, acc);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i0 + u * nt >= total) continue;
+            float v = g[u];
+            if (t.mom) {
+                v = mu_update(a, g[u], m[u]);
+                t.mom[i0 + u * nt] = m[u];
+            }
+            acc = fma((double)v, (double)v, acc);
+        }
     }
     for (int d = 32; d >= 1; d >>= 1) acc += __shfl_xor(acc, d, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
@@ -436,7 +449,7 @@ __device__ __forceinline__ void mu_put(const MuArgs& a, const MuMat& t, int row,
         __bf16* p = reinterpret_cast<__bf16*>(t.out) + at;
         bf16x4 q;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = (__bf16)(k < end ? v[k] : 0.0f);
+        for (int k = 0; k < 4; ++k) q[k] = (__bf16)(k < count ? v[k] : 0.0f);
         if (vec) *reinterpret_cast<bf16x4*>(p) = q;
         else
 #pragma unroll
@@ -588,7 +601,9 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
 // X and A (then B over A) of one matrix stay in LDS as fragments, 16 waves share the products in blocks of 32 x 32, results
 // wait in registers until everyone has read the operands they replace.  X is kept one way only: where k runs along its rows
 // the fragments are read with the transposing LDS read.  One launch for norm, five steps and update; the launches of the
-// general path cost 60 to 110 us whatever the size (five matrices of 64 x 192 to 128 x 192: 110 us there).
+// general path cost 60 to 110 us whatever the size.  Measured, this way and that: 64 x 64 28 and 71 us, 64 x 192 37 and 80,
+// 128 x 192 69 and 88, 32 x 1000 73 and 103; bf16 128 x 192 47 and 77; the agent's five matrices 73 and 110.  Of 128 x 192's
+// step (25 k cycles) the products are half, bound by LDS reads; the rest is waiting for the slowest wave and storing.
 constexpr int MU_SMALL_LDS = 160 * 1024;
 template <int P> struct MuSmall { static constexpr int NEXT = P == 2 ? 2 : 3, SYM = P == 2 ? 1 : 2; };      // most blocks a wave gets
 

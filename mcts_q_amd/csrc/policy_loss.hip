@@ -10,11 +10,15 @@
 //     thread turns them into the coefficient.  Where U vectors a lane hold the whole row (HOLD), the exponentials stay in
 //     registers and the gradient is one product per element; longer rows are read a second time, now from the caches.
 //   - rows of at most 256 elements go to groups of 1, 4 or 16 lanes and stay in registers, many rows to a workgroup.
-// Statistics: exponentials and the sums of one lane in fp32 (at most 32 terms between two rescalings), everything joined
-// across lanes, the logarithm, ratio, KL term and loss in fp64: the clip decides on a ratio that two evaluations must agree
-// on.  Rows of weight 0 are padding: their logits, action, and statistics are not read, their outputs are exactly 0.
+// Statistics: exponentials in fp32, added four at a time in fp32 and beyond that in fp64 (a sum of fp32 steps shows where one
+// action has nearly all the probability and its logarithm is small); the joins across lanes, the logarithm, ratio, KL term
+// and loss in fp64: the clip decides on a ratio that two evaluations must agree on.
+// Rows of weight 0 are padding: their logits, action, and statistics are not read, their outputs are exactly 0.
 // An action outside [0, V) on a row that has weight makes that row's outputs and the loss NaN; nothing is read for it.
 // Sums are joined in a fixed order: the same inputs give the same bits.
+// Measured (a large copy reaches 5.15 TB/s, a read 6.05): log-probabilities of 4096 x 32000 bf16 5.2 TB/s, fp32 5.8; policy
+// loss and gradient of 8192 x 16000 bf16 5.0, 4096 x 32000 fp32 5.2, 4096 x 131072 bf16 with a third of the rows padding
+// 404 us (343 at the copy's rate); preference loss of 16 x 511 x 50257 bf16 392 us (359 with its second reading).
 #include <float.h>
 #include <math.h>
 
@@ -159,15 +163,26 @@ __device__ __forceinline__ float exp_diff_sum(float x, float m) {
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
 
-template <int VE>
-__device__ __forceinline__ void accumulate(const float* f, float& m, float& s) {
-    float bm = f[0];
+// sum of exp(f - ref) over N values, left in f: four at a time in fp32, those sums in fp64
+template <int N>
+__device__ __forceinline__ double sum_exp(float* f, float ref) {
+    double s = 0.0;
 #pragma unroll
-    for (int j = 1; j < VE; ++j) bm = fmaxf(bm, f[j]);
-    const float nm = fmaxf(m, bm), ref = finite_or_zero(nm);
-    s *= exp_diff_sum(m, ref);                          // m = -inf: the factor is 0, and so is s
+    for (int j = 0; j < N; j += 4) {
 #pragma unroll
-    for (int j = 0; j < VE; ++j) s += exp_diff_sum(f[j], ref);
+        for (int k = j; k < j + 4; ++k) f[k] = exp_diff_sum(f[k], ref);
+        s += (double)((f[j] + f[j + 1]) + (f[j + 2] + f[j + 3]));
+    }
+    return s;
+}
+template <int N>
+__device__ __forceinline__ void accumulate(float* f, float& m, double& s) {
+    float nm = m;
+#pragma unroll
+    for (int j = 0; j < N; ++j) nm = fmaxf(nm, f[j]);
+    const float ref = finite_or_zero(nm);
+    s *= (double)exp_diff_sum(m, ref);                  // m = -inf: the factor is 0, and so is s
+    s += sum_exp<N>(f, ref);
     m = nm;
 }
 
@@ -383,7 +398,7 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a)
         float ex[HOLD ? U * VE : 1], lane_m = 0.0f;
         if constexpr (MODE != MODE_GRAD) {
             if (tid == 0) za = Elem<T>::load(rv.base, act);
-            float s = 0.0f;
+            double sd = 0.0;
             if constexpr (HOLD) {
                 u32x4 y[U];
 #pragma unroll
@@ -395,9 +410,7 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a)
                 for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], ex + u * VE);
 #pragma unroll
                 for (int j = 0; j < U * VE; ++j) m = fmaxf(m, ex[j]);
-                const float ref = finite_or_zero(m);
-#pragma unroll
-                for (int j = 0; j < U * VE; ++j) s += ex[j] = exp_diff_sum(ex[j], ref);
+                sd = sum_exp<U * VE>(ex, finite_or_zero(m));
                 lane_m = m;
             } else for (int64_t v0 = tid; v0 < rv.nvec; v0 += U * NT) {
                 u32x4 y[U];
@@ -409,9 +422,8 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a)
                 float f[U * VE];
 #pragma unroll
                 for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], f + u * VE);
-                accumulate<U * VE>(f, m, s);
+                accumulate<U * VE>(f, m, sd);
             }
-            double sd = (double)s;
             join_lanes<64>(m, sd);
             if constexpr (RW > 1) {
                 if (lane == 0) { s_m[wave] = m; s_s[wave] = sd; }
@@ -506,7 +518,7 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
         const int64_t act = w != 0.0f ? row_action(a, row) : 0;
         const bool bad = act < 0 || act >= a.V, live = w != 0.0f && !bad;
         const char* z = a.z + row_offset(a, row, a.z_so, a.z_si) * (int64_t)sizeof(T);
-        float x[EPL], m = -INFINITY, lane_m = 0.0f, inv, coef = 0.0f, za = 0.0f, s = 0.0f;
+        float x[EPL], m = -INFINITY, lane_m = 0.0f, inv, coef = 0.0f, za = 0.0f;
 #pragma unroll
         for (int k = 0; k < EPL; ++k) {
             x[k] = -INFINITY;
@@ -517,11 +529,11 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
         if constexpr (MODE != MODE_GRAD) {
             if (live) za = Elem<T>::load(z, act);
             const float ref = finite_or_zero(m);
+            double sd = 0.0;
             lane_m = m;
 #pragma unroll
             for (int k = 0; k < EPL; ++k)
-                if (k * G < a.V) s += x[k] = exp_diff_sum(x[k], ref);
-            double sd = (double)s;
+                if (k * G < a.V) sd += (double)(x[k] = exp_diff_sum(x[k], ref));
             join_lanes<G>(m, sd);
             inv = fast_rcp((float)sd);
             if (in && g == 0) {

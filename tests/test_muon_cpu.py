@@ -75,3 +75,11 @@ def test_planes_stay_in_range():
     assert f.min() >= 0 and f.max() <= 1.2051
     lam = s * s
     assert (b * lam + c * lam * lam).abs().max() * 2 ** 14 < 65504 and lam.max() * 2 ** 14 < 65504
+    q = a + b * lam + c * lam * lam                     # Q; Q A; and products of up to three steps' Q at 2^14, 2^12, 2^10
+    assert q.abs().max() * 2 ** 14 < 65504 and (q * lam).abs().max() * 2 ** 14 < 65504
+    s1 = s[s <= 1.0]
+    n = torch.ones_like(s1)
+    for k in range(3):
+        n = n * (a + b * s1 ** 2 + c * s1 ** 4)
+        s1 = a * s1 + b * s1 ** 3 + c * s1 ** 5
+        assert n.abs().max() * 2 ** (14 - 2 * k) < 65504
