@@ -634,7 +634,7 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
         a.seq_logp[p] = (float)Sc; a.seq_logp[p + a.P] = (float)Sr;
         a.margin[p] = live ? (float)h : 0.0f;
         a.seq_coef[p] = (float)c; a.seq_coef[p + a.P] = (float)-c;
-        l = sw * ((1.0 - a.smooth) * up + a.smooth * down);
+        l = sw * ((1.0 - a.smooth) * up + (a.smooth > 0.0 ? a.smooth * down : 0.0));      // h may be infinite
         if (h != h) l = h * sw;
         if (!live) l = 0.0;
     }

@@ -291,6 +291,33 @@ def test_preference_padding_pairs():
     assert float(none["loss"]) == 0 and not none["dlogits"].any()
 
 
+def test_preference_weights_and_impossible_tokens():
+    """Fractional and negative row weights enter the sums; a rejected sequence that holds a token of probability 0 is as
+    good as told apart (loss 0), a preferred one is an infinite loss with a finite gradient."""
+    from mcts_q_amd.policyloss import preference_loss
+    P, T, V = 3, 4, 40
+    z, a, g = _make((2 * P, T), V, torch.float32, seed=21)
+    w = torch.randn(2 * P, T, generator=g, device="cuda")
+    ref = torch.randn(2 * P, generator=g, device="cuda")
+    r = preference_loss(z, a, ref, weight=w, beta=0.3)
+    logp = _logp64(z, a).requires_grad_(True)
+    S = (w.double() * logp).sum(1)
+    h = 0.3 * ((S[:P] - ref[:P].double()) - (S[P:] - ref[P:].double()))
+    loss = -torch.nn.functional.logsigmoid(h).mean()
+    loss.backward()
+    eS = float(w.abs().sum(1).max()) * K * U
+    assert ((r["seq_logp"].double() - S).abs() <= eS + U * S.abs()).all()
+    assert abs(float(r["loss"]) - float(loss.detach())) <= 0.6 * eS + U * float(loss.detach())
+    _check_grad_with(r["dlogits"], z, a, logp.grad, w != 0, w.double().abs() * 0.3 / P * 0.25 * 0.6 * eS)
+    z[P + 1, 2, a[P + 1, 2]] = float("-inf")
+    r = preference_loss(z, a, ref, beta=0.3)
+    assert float(r["margin"][1]) == math.inf and torch.isfinite(r["loss"]).all() and not r["dlogits"][1].any()
+    assert not r["dlogits"][P + 1].any()
+    z[0, 1, a[0, 1]] = float("-inf")
+    r = preference_loss(z, a, ref, beta=0.3)
+    assert float(r["margin"][0]) == -math.inf and float(r["loss"]) == math.inf and torch.isfinite(r["dlogits"]).all()
+
+
 def test_gradients_against_differences():
     """Central differences of the reported loss along random directions of fp32 logits: step s, the loss changes by
     s <g, v> with an error of s^2 (third derivatives of O(1)) and of the loss's own K u / s."""
