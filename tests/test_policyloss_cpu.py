@@ -60,3 +60,12 @@ def test_no_cpu_fallback():
               lambda: preference_loss(z, a, torch.zeros(2))):
         with pytest.raises(MctsqError):
             f()
+
+
+def test_sizes_whose_products_leave_64_bits():
+    """2 * 2^30 * 2^33 = 2^64 rows would count as none; 2^59 * 2^3 bytes likewise."""
+    for pairs, tokens in ((1 << 30, 1 << 33), (1 << 59, 1), (1, 1 << 62)):
+        assert lib.mctsq_preference_loss_workspace_bytes(pairs, tokens) < 0
+        assert b"out of range" in lib.mctsq_last_error()
+        assert _pref(pairs=pairs, T=tokens, wsb=1 << 20) < 0
+        assert b"out of range" in lib.mctsq_last_error()
