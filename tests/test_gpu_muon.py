@@ -61,7 +61,7 @@ def test_large_tiles_and_many_matrices(dtype):
     from mcts_q_amd.muon import orthogonalize
     x = _rand((9, 900, 1000), 5, dtype)                       # 9 * 36 = 324 tiles on and below the diagonals
     _close(orthogonalize(x), _truth(x), TOL[dtype])
-    y = _rand((45, 24, 40), 6, dtype)
+    y = _rand((75, 24, 40), 6, dtype)
     _close(orthogonalize(y), _truth(y), TOL[dtype])
     z = _rand((8, 1000, 900), 7, dtype)
     _close(orthogonalize(z), _truth(z), TOL[dtype])
@@ -78,10 +78,17 @@ def test_every_plan_and_tile(shape, dtype):
     _close(orthogonalize(x), _truth(x), TOL[dtype])
 
 
+@pytest.mark.parametrize("shape", [(3, 40000), (20000, 40), (1, 65536)])
+def test_long_and_thin(shape):
+    from mcts_q_amd.muon import orthogonalize
+    x = _rand(shape, 13)
+    _close(orthogonalize(x), _truth(x), TOL[torch.float32])
+
+
 def test_a_mixed_list_of_large_and_small():
-    """One step of 23 matrices (more than one launch group) from 8 x 9 to 1500 x 600, a NaN in one of them."""
+    """One step of 43 matrices (more than one launch group) from 8 x 9 to 1500 x 600, a NaN in one of them."""
     from mcts_q_amd.muon import DeviceMuon
-    shapes = [(8, 9), (1500, 600), (600, 1500), (64, 64), (700, 700)] + [(32 + i, 100) for i in range(18)]
+    shapes = [(8, 9), (1500, 600), (600, 1500), (64, 64), (700, 700)] + [(32 + i, 100) for i in range(38)]
     params = [_rand(s, i) for i, s in enumerate(shapes)]
     start = [p.double() for p in params]
     grads = [_rand(s, 50 + i) for i, s in enumerate(shapes)]
@@ -108,6 +115,8 @@ def test_known_results():
     assert ((one.flatten().double().cpu() - f * torch.tensor([1.0, -1.0, 1.0])).abs() <= TOL[torch.float32] + 5e-4).all()
     for dt in (torch.float32, torch.bfloat16):
         assert not orthogonalize(torch.zeros(100, 30, dtype=dt, device="cuda")).any()
+        assert not orthogonalize(torch.zeros(3, 300, 400, dtype=dt, device="cuda"), eps=1e-300).any()
+        assert not orthogonalize(torch.zeros(3, 5, dtype=dt, device="cuda"), eps=1e-300).any()
     s = torch.linalg.svdvals(orthogonalize(_rand((300, 500), 3)).double())
     assert s.max() < 1.21 and s.min() > 0.3
 
