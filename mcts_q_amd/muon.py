@@ -7,6 +7,8 @@ with operands of 11 bits (directions weaker than 2^-11 of the strongest are lost
 stream of the tensors' device; nothing synchronises."""
 from __future__ import annotations
 
+from bisect import bisect_left
+
 import torch
 
 from ._lib import MctsqError, MuonMatrix, lib, on_device, ptr, stream_ptr
@@ -88,8 +90,9 @@ class DeviceMuon:
 
     f by `adjust`: "spectral" sqrt(max(1, rows / cols)), "rms" 0.2 sqrt(max(rows, cols)), "none" 1.  A parameter is
     [rows, cols] or a stack [count, rows, cols] of matrices, rows contiguous.  Gradients are fp32 or bf16, all of one type.
-    `momentum_buffers` (fp32, contiguous, one per parameter) is the state; the workspace is kept, so steps of one instance
-    belong on one stream at a time (two graphs captured from one instance must not run at once)."""
+    They share no memory with the parameters or the state: `momentum_buffers` (fp32, contiguous, one per parameter).  The
+    workspace is kept, so steps of one instance belong on one stream at a time (two graphs captured from one instance must
+    not run at once), and an instance has to live as long as the graphs captured from it."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, eps=1e-7, adjust="spectral",
                  momentum_buffers=None):
@@ -121,6 +124,12 @@ class DeviceMuon:
             if m.shape != p.shape or m.dtype != torch.float32 or m.device != p.device or not m.is_contiguous():
                 raise ValueError(f"momentum_buffers[{i}]: expected contiguous fp32 {tuple(p.shape)} on {p.device}")
         self.momentum_buffers = list(momentum_buffers)
+        # what a step writes, in the order of memory (of strided parameters their bounds may interleave: the starts alone)
+        self._starts = {p.data_ptr() for p in params}
+        written = sorted(_span(t) for t in self.momentum_buffers + [p for p in params if p.is_contiguous()])
+        if any(b0 < a1 for (_, a1), (b0, _) in zip(written, written[1:])):
+            raise ValueError("momentum_buffers: must share no memory with each other or the parameters")
+        self._first, self._last = [a for a, _ in written], [b for _, b in written]
         mats, self._spans = [], []
         for p, m in zip(params, self.momentum_buffers):
             ps, ms = _slices(p), _slices(m)
@@ -139,10 +148,14 @@ class DeviceMuon:
         dt = grads[0].dtype
         if dt not in _DTYPE:
             raise ValueError(f"grads: expected fp32 or bf16, got {dt}")
-        for i, (g, p, (at, k)) in enumerate(zip(grads, self.params, self._spans)):
+        for i, (g, p, (at, _)) in enumerate(zip(grads, self.params, self._spans)):
             if g.shape != p.shape or g.dtype != dt or g.device != self.device or not _is_matrix(g):
                 raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {dt} on {self.device} with contiguous rows, got "
                                  f"{tuple(g.shape)} {g.dtype} with strides {g.stride()} on {g.device}")
+            a, b = _span(g)
+            k = bisect_left(self._first, b)                  # the last written range that starts before the gradient's end
+            if (k and self._last[k - 1] > a) or a in self._starts:
+                raise ValueError(f"grads[{i}]: must share no memory with the parameters or the momentum")
             ld = _ld(g)
             for j, q in enumerate(_slices(g)):
                 self._mats[at + j].d_x, self._mats[at + j].ldx = q, ld

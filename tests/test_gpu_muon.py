@@ -259,3 +259,28 @@ def test_state_and_refusals():
             bad()
     with pytest.raises(MctsqError):
         orthogonalize(z, eps=0.0)
+
+
+def test_shared_memory_is_refused():
+    """A gradient that is the momentum would change between its two readings; one buffer for two states would mix them."""
+    from mcts_q_amd.muon import DeviceMuon
+    flat = torch.zeros(6 * 48, device="cuda")
+    a, b, m, n, g, h = [flat[48 * i:48 * i + 48].view(6, 8) for i in range(6)]
+    for bad in ([m, m], [m, a], [m, flat[120:168].view(6, 8)]):
+        with pytest.raises(ValueError):
+            DeviceMuon([a, b], momentum_buffers=bad)
+    opt = DeviceMuon([a, b], momentum_buffers=[m, n])
+    for bad in ([m, h], [g, n], [a, h], [g, a], [flat[72:120].view(6, 8), h], [flat[168:216].view(6, 8), h]):
+        with pytest.raises(ValueError):
+            opt.step(bad)
+    assert not flat.any()
+    g.copy_(_rand((6, 8), 1))
+    opt.step([g, g])                                        # read only: one gradient for two matrices is fine
+    assert torch.equal(a, b) and a.any() and not h.any()
+    wide = torch.zeros(6, 20, device="cuda")
+    strided = DeviceMuon([wide[:, :8]])
+    with pytest.raises(ValueError):
+        strided.step([wide[:, :8]])
+    wide[:, 8:16] = g
+    strided.step([wide[:, 8:16]])                           # interleaved rows share nothing
+    assert torch.equal(wide[:, :8], a) and torch.equal(wide[:, 8:16], g) and not wide[:, 16:].any()
