@@ -10,13 +10,13 @@
 //     thread turns them into the coefficient.  Where U vectors a lane hold the whole row (HOLD), the exponentials stay in
 //     registers and the gradient is one product per element; longer rows are read a second time, now from the caches.
 //   - rows of at most 256 elements go to groups of 1, 4 or 16 lanes and stay in registers, many rows to a workgroup.
-// Statistics: exponentials in fp32, added four at a time in fp32 and beyond that in fp64 (a sum of fp32 steps shows where one
-// action has nearly all the probability and its logarithm is small); the joins across lanes, the logarithm, ratio, KL term
+// Statistics: exponentials in fp32, added in fp64, of many 16-bit rows four at a time in fp32 first (a sum of fp32 steps shows
+// where one action has nearly all the probability and its logarithm is small; see sum_exp); the joins across lanes, the logarithm, ratio, KL term
 // and loss in fp64: the clip decides on a ratio that two evaluations must agree on.
 // Rows of weight 0 are padding: their logits, action, and statistics are not read, their outputs are exactly 0.
 // An action outside [0, V) on a row that has weight makes that row's outputs and the loss NaN; nothing is read for it.
 // Sums are joined in a fixed order: the same inputs give the same bits.
-// Measured (a large copy reaches 5.15 TB/s, a read 6.05): log-probabilities of 4096 x 32000 bf16 5.2 TB/s, fp32 5.8; policy
+// Measured (a large copy reaches 5.15 TB/s, a read 6.05): log-probabilities of 4096 x 32000 bf16 5.9 TB/s, fp32 5.4; policy
 // loss and gradient of 8192 x 16000 bf16 5.0, 4096 x 32000 fp32 5.2, 4096 x 131072 bf16 with a third of the rows padding
 // 404 us (343 at the copy's rate); preference loss of 16 x 511 x 50257 bf16 392 us (359 with its second reading).
 #include <float.h>
@@ -161,28 +161,62 @@ __device__ __forceinline__ float exp_diff_sum(float x, float m) {
     const float d = x - m;
     return fast_exp2(fmaf(d, LOG2E, d * LOG2E_LO));
 }
+// The same, and in r what its argument lost in rounding (3e-7 of the exponential at x - m = -10): exp(x - m) = e (1 + r log 2).
+// Far below, where e is 0, r must not be NaN.
+constexpr float LN2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp_diff_rest(float x, float m, float& r) {
+    const float d = __builtin_elementwise_maximum(x - m, -200.0f), t = d * LOG2E_LO, y = fmaf(d, LOG2E, t);   // NaN stays NaN
+    r = fmaf(d, LOG2E, -y) + t;
+    return fast_exp2(y);
+}
+template <bool ACC>
+__device__ __forceinline__ double exp_factor(float x, float m) {
+    if constexpr (!ACC) return (double)exp_diff_sum(x, m);
+    float r;
+    const float e = exp_diff_rest(x, m, r);
+    return (double)e * fma((double)r, (double)LN2, 1.0);
+}
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// sum of exp(f - ref) over N values, left in f: four at a time in fp32, those sums in fp64
-template <int N>
+// Sum of exp(f - ref) over N values, left in f: four at a time in fp32, those sums in fp64 -- or, ACC, each in fp64 together
+// with what the exponentials' arguments lost.  Two log-probabilities' difference, rows of 32000 to 81298, rms against 64 bits:
+// 2.9e-8, ACC 1.0e-8 (what is left is the exponential instruction's own).  ACC is for fp32 logits (4096 x 32000: 92 -> 97 us,
+// with the gradient 202 -> 198) and for at most a row per CU, where nothing is bound by it and no number of rows averages the
+// errors; many 16-bit rows would pay 25 % (45 -> 56 us).
+template <int N, bool ACC>
 __device__ __forceinline__ double sum_exp(float* f, float ref) {
-    double s = 0.0;
+    double s = 0.0, t = 0.0;
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
+        if constexpr (ACC) {
+            float c = 0.0f;
 #pragma unroll
-        for (int k = j; k < j + 4; ++k) f[k] = exp_diff_sum(f[k], ref);
-        s += (double)((f[j] + f[j + 1]) + (f[j + 2] + f[j + 3]));
+            for (int k = j; k < j + 4; ++k) {
+                float r;
+                f[k] = exp_diff_rest(f[k], ref, r);
+                c = fmaf(f[k], r, c);
+            }
+            s += (double)f[j];
+            t += (double)f[j + 1];
+            s += (double)f[j + 2];
+            t += (double)f[j + 3];
+            s += (double)(c * LN2);
+        } else {
+#pragma unroll
+            for (int k = j; k < j + 4; ++k) f[k] = exp_diff_sum(f[k], ref);
+            s += (double)((f[j] + f[j + 1]) + (f[j + 2] + f[j + 3]));
+        }
     }
-    return s;
+    return ACC ? s + t : s;
 }
-template <int N>
+template <int N, bool ACC>
 __device__ __forceinline__ void accumulate(float* f, float& m, double& s) {
     float nm = m;
 #pragma unroll
     for (int j = 0; j < N; ++j) nm = fmaxf(nm, f[j]);
     const float ref = finite_or_zero(nm);
-    s *= (double)exp_diff_sum(m, ref);                  // m = -inf: the factor is 0, and so is s
-    s += sum_exp<N>(f, ref);
+    s *= exp_factor<ACC>(m, ref);                       // m = -inf: the factor is 0, and so is s
+    s += sum_exp<N, ACC>(f, ref);
     m = nm;
 }
 
@@ -204,12 +238,13 @@ __device__ __forceinline__ double lane_f64(double v, int l) {
 }
 
 // a pair (m, s) as it counts under the joint maximum M
+template <bool ACC>
 __device__ __forceinline__ double rescaled(float m, double s, float M) {
-    const double r = s * (double)exp_diff_sum(m, finite_or_zero(M));
+    const double r = s * exp_factor<ACC>(m, finite_or_zero(M));
     return m > -INFINITY || s != s ? r : 0.0;            // an empty set, or one of -inf only; NaN stays
 }
 // join over groups of W = 1, 4, 16 or 64 consecutive lanes: every lane gets the group's max and sum
-template <int W>
+template <int W, bool ACC>
 __device__ __forceinline__ void join_lanes(float& m, double& s) {
     if constexpr (W == 1) return;
     float M = m;
@@ -218,7 +253,7 @@ __device__ __forceinline__ void join_lanes(float& m, double& s) {
         M = fmaxf(M, dpp_row<0x4E>(M));
     } else if constexpr (W > 1) M = row16_max_dpp(M);
     if constexpr (W == 64) M = fmaxf(fmaxf(lane_f32(M, 0), lane_f32(M, 16)), fmaxf(lane_f32(M, 32), lane_f32(M, 48)));
-    s = rescaled(m, s, M);
+    s = rescaled<ACC>(m, s, M);
     if constexpr (W == 4) {
         s += dpp_f64<0xB1>(s);
         s += dpp_f64<0x4E>(s);
@@ -365,7 +400,7 @@ __device__ __forceinline__ void fill_row(char* out, int64_t V, float v, int tid,
 }
 
 // Long rows: RW waves to a row; one row at a time, or four rows to a workgroup where a wave has its own (RW = 1).
-template <typename T, int RW, int U, bool HOLD, int MODE>
+template <typename T, int RW, int U, bool HOLD, int MODE, bool ACC>
 __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a) {
     constexpr int NT = RW * 64, RPB = RW == 1 ? 4 : 1, VE = Elem<T>::VE;
     static_assert(!HOLD || MODE == MODE_POLICY, "only the one-launch gradient keeps a row");
@@ -410,7 +445,7 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a)
                 for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], ex + u * VE);
 #pragma unroll
                 for (int j = 0; j < U * VE; ++j) m = fmaxf(m, ex[j]);
-                sd = sum_exp<U * VE>(ex, finite_or_zero(m));
+                sd = sum_exp<U * VE, ACC>(ex, finite_or_zero(m));
                 lane_m = m;
             } else for (int64_t v0 = tid; v0 < rv.nvec; v0 += U * NT) {
                 u32x4 y[U];
@@ -422,15 +457,15 @@ __global__ __launch_bounds__(RW == 1 ? 256 : RW * 64) void row_kernel(RowArgs a)
                 float f[U * VE];
 #pragma unroll
                 for (int u = 0; u < U; ++u) Elem<T>::unpack(y[u], f + u * VE);
-                accumulate<U * VE>(f, m, sd);
+                accumulate<U * VE, ACC>(f, m, sd);
             }
-            join_lanes<64>(m, sd);
+            join_lanes<64, ACC>(m, sd);
             if constexpr (RW > 1) {
                 if (lane == 0) { s_m[wave] = m; s_s[wave] = sd; }
                 __syncthreads();
                 m = (lane & 15) < RW ? s_m[lane & 15] : -INFINITY;
                 sd = (lane & 15) < RW ? s_s[lane & 15] : 0.0;
-                join_lanes<16>(m, sd);
+                join_lanes<16, ACC>(m, sd);
             }
             inv = fast_rcp((float)sd);
             if (tid == 0) {
@@ -533,8 +568,12 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
             lane_m = m;
 #pragma unroll
             for (int k = 0; k < EPL; ++k)
-                if (k * G < a.V) sd += (double)(x[k] = exp_diff_sum(x[k], ref));
-            join_lanes<G>(m, sd);
+                if (k * G < a.V) {
+                    float r;
+                    x[k] = exp_diff_rest(x[k], ref, r);
+                    sd += (double)x[k] * fma((double)r, (double)LN2, 1.0);
+                }
+            join_lanes<G, true>(m, sd);
             inv = fast_rcp((float)sd);
             if (in && g == 0) {
                 if (live) loss += row_result<MODE>(a, row, w, za, m, sd, inv, coef);
@@ -647,7 +686,7 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
 
 constexpr int64_t MAX_GRID = 16384;
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool ACC>
 static int64_t launch_rows(const RowArgs& a, hipStream_t st) {
     int64_t grid;
 #define MCTSQ_ROWS(nt, per, ...)                                                                  \
@@ -677,40 +716,43 @@ static int64_t launch_rows(const RowArgs& a, hipStream_t st) {
     // vectors of a row: at its worst alignment, unless every row starts on a vector
     const int64_t es = sizeof(T), starts = (int64_t)((uintptr_t)a.z & 15) | ((a.z_si | (a.one_group ? 0 : a.z_so)) * es & 15);
     const int64_t nv = (a.V + (starts ? 2 * Elem<T>::VE - 2 : Elem<T>::VE - 1)) / Elem<T>::VE;
-    if (nv <= 64) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 1, MODE == MODE_POLICY, MODE>);
-    if (nv <= 128) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 2, MODE == MODE_POLICY, MODE>);
+    if (nv <= 64) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 1, MODE == MODE_POLICY, MODE, ACC>);
+    if (nv <= 128) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 2, MODE == MODE_POLICY, MODE, ACC>);
     if constexpr (MODE == MODE_POLICY) {
-        if (nv <= 256) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, true, MODE>);
-        if (nv <= 512) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 8, true, MODE>);
-        if (nv <= 1024) MCTSQ_ROWS(128, 1, row_kernel<T, 2, 8, true, MODE>);
-        if (nv <= 2048) MCTSQ_ROWS(256, 1, row_kernel<T, 4, 8, true, MODE>);
+        if (nv <= 256) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, true, MODE, ACC>);
+        if (nv <= 512) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 8, true, MODE, ACC>);
+        if (nv <= 1024) MCTSQ_ROWS(128, 1, row_kernel<T, 2, 8, true, MODE, ACC>);
+        if (nv <= 2048) MCTSQ_ROWS(256, 1, row_kernel<T, 4, 8, true, MODE, ACC>);
         if (nv <= 4096) {
-            if constexpr (sizeof(T) == 4) MCTSQ_ROWS(512, 1, row_kernel<T, 8, 8, true, MODE>);
-            else MCTSQ_ROWS(512, 1, row_kernel<T, 8, 4, false, MODE>);
+            if constexpr (sizeof(T) == 4) MCTSQ_ROWS(512, 1, row_kernel<T, 8, 8, true, MODE, ACC>);
+            else MCTSQ_ROWS(512, 1, row_kernel<T, 8, 4, false, MODE, ACC>);
         }
-        if (nv <= 8192) MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 8, true, MODE>);
-        MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 4, false, MODE>);
+        if (nv <= 8192) MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 8, true, MODE, ACC>);
+        MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 4, false, MODE, ACC>);
     } else if constexpr (MODE == MODE_LOGP) {
         // one pass, few registers: a wave per row up to 16 KB, four above (32000 bf16: 4 waves 5190 GB/s, 16 waves 3480) --
         // unless there are too few rows to fill the chip that way, when the whole workgroup shortens each (64 rows of
         // 32000: 10.4 us against 15.7)
-        if (a.rows * (bytes <= 16384 ? 1 : 4) < 2048 && nv > 256) MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 4, false, MODE>);
-        if (bytes <= 16384) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, false, MODE>);
-        MCTSQ_ROWS(256, 1, row_kernel<T, 4, 4, false, MODE>);
+        if (a.rows * (bytes <= 16384 ? 1 : 4) < 2048 && nv > 256) MCTSQ_ROWS(1024, 1, row_kernel<T, 16, 4, false, MODE, ACC>);
+        if (bytes <= 16384) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, false, MODE, ACC>);
+        MCTSQ_ROWS(256, 1, row_kernel<T, 4, 4, false, MODE, ACC>);
     } else {
         // statistics are known: a plain sweep
-        if (bytes <= 8192) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, false, MODE>);
-        if (bytes <= 32768) MCTSQ_ROWS(128, 1, row_kernel<T, 2, 4, false, MODE>);
-        MCTSQ_ROWS(512, 1, row_kernel<T, 8, 4, false, MODE>);
+        if (bytes <= 8192) MCTSQ_ROWS(256, 4, row_kernel<T, 1, 4, false, MODE, ACC>);
+        if (bytes <= 32768) MCTSQ_ROWS(128, 1, row_kernel<T, 2, 4, false, MODE, ACC>);
+        MCTSQ_ROWS(512, 1, row_kernel<T, 8, 4, false, MODE, ACC>);
     }
 #undef MCTSQ_ROWS
 }
 
 template <int MODE>
 static int64_t launch_rows(int dtype, const RowArgs& a, hipStream_t st) {
-    if (dtype == DT_F32) return launch_rows<float, MODE>(a, st);
-    if (dtype == DT_BF16) return launch_rows<__bf16, MODE>(a, st);
-    return launch_rows<_Float16, MODE>(a, st);
+    if (dtype == DT_F32) return launch_rows<float, MODE, MODE != MODE_GRAD>(a, st);
+    if constexpr (MODE != MODE_GRAD)
+        if (a.rows <= 256)
+            return dtype == DT_BF16 ? launch_rows<__bf16, MODE, true>(a, st) : launch_rows<_Float16, MODE, true>(a, st);
+    if (dtype == DT_BF16) return launch_rows<__bf16, MODE, false>(a, st);
+    return launch_rows<_Float16, MODE, false>(a, st);
 }
 
 // shapes and strides every entry point shares; fills the logits part of `a`

@@ -318,6 +318,26 @@ def test_preference_weights_and_impossible_tokens():
     assert float(r["margin"][0]) == -math.inf and float(r["loss"]) == math.inf and torch.isfinite(r["dlogits"]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [5, 200, 700, 4000, 32000, 81298])
+def test_single_rows_that_are_all_but_equal(dtype, V):
+    """One pair of one token each: the margin is a small difference of two log-probabilities.  Of calls of few rows an
+    exponential is exp2 of an argument whose rounding is made good, so it is off by the instruction's step, 2 u; everything
+    after it is fp64.  A term meets at most five of them: its own, two where a lane's maximum moves (three sweeps take 81298
+    elements), the join of the lanes, the join of the waves: 10 u.  x - m rounds by |x - m| u, in fp32 by at most 40 u (a
+    term further below counts for nothing); of 16-bit logits it is exact but for |x| < 2^-10, a few in 10^4 elements whose
+    terms are less than a tenth of the mean: far below u.  The margin rounds once."""
+    from mcts_q_amd.policyloss import preference_loss
+    bound = (50 if dtype == torch.float32 else 10) * U
+    for seed in range(8):
+        z, a, g = _make((2, 1), V, dtype, seed=seed)
+        logp = _logp64(z, a)[:, 0]
+        ref = logp.float() + torch.tensor([1e-3, 0.0], device="cuda")
+        h = 0.1 * ((logp[0] - ref[0].double()) - (logp[1] - ref[1].double()))
+        got = preference_loss(z, a, ref, beta=0.1, grad=False)["margin"].double()
+        assert abs(float(got - h)) <= 0.1 * 2 * bound + U * abs(float(h)), (seed, float(got), float(h))
+
+
 def test_gradients_against_differences():
     """Central differences of the reported loss along random directions of fp32 logits: step s, the loss changes by
     s <g, v> with an error of s^2 (third derivatives of O(1)) and of the loss's own K u / s."""
