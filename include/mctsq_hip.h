@@ -294,8 +294,7 @@ int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pairs, int64_
  *                   p <- p (1 - lr weight_decay) - lr f X,  f = 1 (NONE), sqrt(max(1, rows / cols)) (SPECTRAL),
  *                   0.2 sqrt(max(rows, cols)) (RMS: the update's root mean square matches an Adam step's)
  * p = d_out, m = d_momentum (contiguous [rows][cols]) in fp32, g = d_x in grad_dtype.  fp32 matrices and the step are
- * evaluated to fp32 accuracy, bf16 matrices with the products' operands in 11 bits and sums in fp32 (directions weaker than
- * 2^-11 of a matrix's strongest are lost).
+ * evaluated to fp32 accuracy, bf16 matrices likewise with one rounding at the end.
  * ld*: elements between rows.  Sides up to 65536, any number of matrices of any mixture of shapes; the same inputs give the
  * same bits.  A matrix that holds an infinity or NaN becomes NaN.  `mats` is read by the host during the call only; matrices
  * must not overlap.  d_ws: the matching *_workspace_bytes() of the same list, 256-byte aligned; its contents are scratch.

@@ -7,14 +7,14 @@
 // Per step n^2 m + n^3 + 2 n^2 m operations: A and Q are symmetric, only tiles that reach the diagonal or lie below it are
 // computed, and stored to both places.  The bound is the matrix pipe from n = 1024 up, the chain of dependent launches below.
 //
-// Arithmetic.  fp32 matrices go through the two-way fp16 split of this library (device_utils.hpp: split2h): every operand is
-// hi + lo in fp16 scaled by 2^14, products lo hi + hi lo + hi hi accumulate in fp32, i.e. fp32 accuracy at three 16-bit
+// Arithmetic.  Matrices of either type go through the two-way fp16 split of this library (device_utils.hpp: split2h): every
+// operand is hi + lo in fp16 scaled by 2^14, products lo hi + hi lo + hi hi accumulate in fp32, i.e. fp32 accuracy at three 16-bit
 // matrix instructions (a library fp32 product reaches 153 TFLOP/s on this card, the fp16 one 1220).  The scale is safe
 // without looking at the data: |u|_F = 1 bounds every singular value of X_0 by 1, the quintic maps [0, 1.21] into itself, so
 // |X| <= 1.21, |A| <= 1.47, |Q| <= 3.4445 and 3.4445 * 2^14 < 65504.
-// bf16 matrices use the hi plane alone: one matrix instruction per product; X, A and Q are rounded to 11 bits each step,
-// which leaves the result 1.9e-3 to 2.2e-3 off where its rounding to bf16 alone is 1.7e-3.  Directions weaker than 2^-11 of
-// the strongest are lost in those 11 bits (four directions carrying all but 1e-3: 1e-2 to 4e-2 off).
+// bf16 matrices are read exactly and rounded once, at the end: their result is the fp32 one's, rounded.  (The hi planes
+// alone, one instruction per product, round X, A and Q to 11 bits each step and lose every direction weaker than 2^-11 of the
+// strongest: up to 4e-2 off where four directions carry all but 1e-3.  3 x 777 x 2050: 259 us that way, 379 this.)
 // X_0 is never rounded by the normalisation: its planes hold u times a power of two, the rest of the factor (in (1, 2])
 // enters the first step's products in fp32.
 //
@@ -33,12 +33,13 @@
 namespace mctsq {
 
 // Matrices per launch (kernel arguments hold their descriptions).  The agent's largest encoders have 19; 32 costs every launch
-// 0.4 us more (3 x 777 x 2050 bf16: 282 against 275 us).
+// 0.4 us more.
 constexpr int MU_GROUP = 20;
 constexpr int MU_PARTS = 256;       // workgroups that add up one matrix's squares
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float PLANE = 16384.0f, UNPLANE = 1.0f / 16384.0f;        // 2^14
 constexpr int FRAG = 512;           // halves in a fragment
+constexpr int P = 2;                // planes of a matrix: hi and lo
 
 enum { MU_F32 = 0, MU_BF16 = 1 };
 
@@ -50,7 +51,7 @@ struct MuMat {
     const void* x; int64_t ldx;     // gradient, or the matrix to orthogonalise
     float* mom;                     // momentum [rows][cols], NULL: orthogonalise x
     void* out; int64_t ldo;         // parameters (updated in place), or the result
-    _Float16* ws;                   // X0 X1 | XT0 XT1 | A | B, each of `planes` planes
+    _Float16* ws;                   // X old and new, four n x n matrices (MuPlanes), each of two planes
     double* part;                   // MU_PARTS sums of squares
 };
 struct MuArgs {
@@ -157,7 +158,6 @@ __device__ __forceinline__ void mu_scale(const MuMat& t, double eps, double& up,
 __device__ __forceinline__ int64_t frag_at(int row, int k, int K) {
     return ((int64_t)(row >> 4) * (K >> 5) + (k >> 5)) * FRAG + (((row & 15) + 16 * ((k & 31) >> 3)) << 3) + (k & 7);
 }
-template <int P>
 struct MuPlanes {                   // where a matrix's planes are: X twice (old and new), four n x n matrices
     int64_t xs, as;                 // halves from a plane to the next
     _Float16* base;
@@ -166,7 +166,6 @@ struct MuPlanes {                   // where a matrix's planes are: X twice (old
     __device__ _Float16* N(int i) const { return base + 2 * P * xs + i * P * as; }
 };
 
-template <int P>
 __global__ __launch_bounds__(256) void mu_planes_kernel(MuArgs a) {
     __shared__ float tile[64][65];
     const int w = mu_which(a, blockIdx.x);
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(256) void mu_planes_kernel(MuArgs a) {
         }
     }
     __syncthreads();
-    const MuPlanes<P> pl(t);
+    const MuPlanes pl(t);
     const int lane = threadIdx.x & 63, row = lane & 15, k0 = (lane >> 4) * 8;
 #pragma unroll
     for (int f = threadIdx.x >> 6; f < 8; f += 4) {
@@ -230,7 +229,7 @@ __global__ __launch_bounds__(256) void mu_planes_kernel(MuArgs a) {
         }
         _Float16* dst = pl.X(0) + frag_at(bi + rt * 16, bj + kb * 32, t.mp) + lane * 8;
         *reinterpret_cast<f16x8*>(dst) = hi;
-        if (P == 2) *reinterpret_cast<f16x8*>(dst + pl.xs) = lo;
+        *reinterpret_cast<f16x8*>(dst + pl.xs) = lo;
     }
 }
 
@@ -263,7 +262,7 @@ __host__ __device__ inline int mu_tiles(int np, int cols, bool sym) {
 // Three LDS buffers: while block k is multiplied from registers, block k + 1 is read from LDS into a second set of registers,
 // blocks k + 2 and k + 3 are on their way from memory.  The buffers are variables of their own, so that the compiler knows that
 // a read of one does not touch what is being fetched into another.
-template <int P, int TI, int TJ>
+template <int TI, int TJ>
 struct MuTile {
     static constexpr int WI = TI / 32, WJ = TJ / 32;                     // 16 x 16 tiles of a wave
     static constexpr int FI = P * TI / 16, F = FI + P * TJ / 16;         // fragments of a k block: of R, of both
@@ -295,11 +294,11 @@ __device__ __forceinline__ void mu_interleave() {
 // TR: S is given with k along its columns (X itself, in place of its transpose): skt k blocks of 32 columns.  Its fragments
 // are read from LDS transposed, groups of 16 lanes taking four rows of 16; every other octet's rows are fetched four places
 // on, so that such a group finds its 128 bytes in different banks.
-template <int P, int TI, int TJ, bool TR>
+template <int TI, int TJ, bool TR>
 __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtiles, const _Float16* S, int64_t ss, int stiles,
-                                        int KB, int ti, int tj, f32x4 (&acc)[MuTile<P, TI, TJ>::WI][MuTile<P, TI, TJ>::WJ],
+                                        int KB, int ti, int tj, f32x4 (&acc)[MuTile<TI, TJ>::WI][MuTile<TI, TJ>::WJ],
                                         _Float16* b0, _Float16* b1, _Float16* b2) {
-    using C = MuTile<P, TI, TJ>;
+    using C = MuTile<TI, TJ>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave >> 1, wj = wave & 1;
     const int place = TR ? (((lane & 15) ^ ((lane >> 4 & 1) << 2)) + (lane & 48)) * 8 : lane * 8;
@@ -355,12 +354,10 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
     auto multiply = [&](const Frags& f) {
 #pragma unroll
         for (int j = 0; j < C::WJ; ++j) {
-            if constexpr (P == 2) {
 #pragma unroll
-                for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[1][i], f.s[0][j], acc[i][j]);
+            for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[1][i], f.s[0][j], acc[i][j]);
 #pragma unroll
-                for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[0][i], f.s[1][j], acc[i][j]);
-            }
+            for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[0][i], f.s[1][j], acc[i][j]);
 #pragma unroll
             for (int i = 0; i < C::WI; ++i) acc[i][j] = mfma_h(f.r[0][i], f.s[0][j], acc[i][j]);
         }
@@ -376,7 +373,7 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
         fetch(k + 3, free);
         read(other, next);
         multiply(cur);
-        mu_interleave<P * (C::WI + (TR ? 2 : 1) * C::WJ), C::L, (P == 2 ? 3 : 1) * C::WI * C::WJ>();
+        mu_interleave<P * (C::WI + (TR ? 2 : 1) * C::WJ), C::L, 3 * C::WI * C::WJ>();
     };
 #pragma unroll
     for (int i = 0; i < C::WI; ++i)
@@ -403,26 +400,22 @@ __device__ __forceinline__ void mu_tile(const _Float16* R, int64_t rs, int rtile
 
 // four consecutive values along k of one row: stored as hi (and lo), and read back
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-template <int P>
 __device__ __forceinline__ void split4(const float* v, f16x4& h, f16x4& l, float plane = PLANE) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         h[r] = (_Float16)(v[r] * plane);
-        l[r] = P == 2 ? (_Float16)(v[r] * plane - (float)h[r]) : (_Float16)0.0f;
+        l[r] = (_Float16)(v[r] * plane - (float)h[r]);
     }
 }
-template <int P>
 struct Quad4 { f16x4 p[P]; };
-template <int P>
-__device__ __forceinline__ Quad4<P> plane_load(const _Float16* at, int64_t ps) {
-    Quad4<P> q;
+__device__ __forceinline__ Quad4 plane_load(const _Float16* at, int64_t ps) {
+    Quad4 q;
 #pragma unroll
     for (int p = 0; p < P; ++p) q.p[p] = *reinterpret_cast<const f16x4*>(at + p * ps);
     return q;
 }
-template <int P>
-__device__ __forceinline__ float plane_value(const Quad4<P>& q, int r) {
-    return (P == 2 ? (float)q.p[0][r] + (float)q.p[P - 1][r] : (float)q.p[0][r]) * UNPLANE;
+__device__ __forceinline__ float plane_value(const Quad4& q, int r) {
+    return ((float)q.p[0][r] + (float)q.p[1][r]) * UNPLANE;
 }
 
 // `count` (at most four; four where vec is set) results in a row of the caller's matrix, from column c on
@@ -459,9 +452,9 @@ __device__ __forceinline__ void mu_put(const MuArgs& a, const MuMat& t, int row,
     }
 }
 
-template <int P, int TI, int TJ, int ST>
+template <int TI, int TJ, int ST>
 __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
-    using C = MuTile<P, TI, TJ>;
+    using C = MuTile<TI, TJ>;
     __shared__ __attribute__((aligned(16))) _Float16 b0[C::BUF], b1[C::BUF], b2[C::BUF];
     constexpr bool sym = ST == ST_SYM || ST == ST_POLY;
     const int w = mu_which(a, blockIdx.x), n = mu_tiles<TI, TJ>(a.mat[w].np, sym ? a.mat[w].np : a.mat[w].mp, sym);
@@ -470,7 +463,7 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
     const int lb = blockIdx.x - a.first[w], q = n >> 3, rest = n & 7, x = lb & 7;
     const int b = x * q + (x < rest ? x : rest) + (lb >> 3);
     const MuMat& t = a.mat[w];
-    const MuPlanes<P> pl(t);
+    const MuPlanes pl(t);
     int ti, tj;
     {
         const int nti = (t.np + TI - 1) / TI, ntj = (t.mp + TJ - 1) / TJ;
@@ -489,8 +482,8 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
         const bool gram = ST == ST_SYM && g.r < 0;                        // X X^T: k runs along m
         const _Float16 *R = gram ? pl.X(g.cur) : pl.N(g.r), *S = gram ? pl.X(g.cur) : pl.N(g.s);
         const int64_t ps = gram ? pl.xs : pl.as;
-        mu_tile<P, TI, TJ, false>(R, ps, nt, S, ps, nt, (gram ? t.mp : t.np) / 32, ti, tj, acc, b0, b1, b2);
-    } else mu_tile<P, TI, TJ, true>(pl.N(g.r), pl.as, nt, pl.X(g.cur), pl.xs, mt, t.np / 32, ti, tj, acc, b0, b1, b2);
+        mu_tile<TI, TJ, false>(R, ps, nt, S, ps, nt, (gram ? t.mp : t.np) / 32, ti, tj, acc, b0, b1, b2);
+    } else mu_tile<TI, TJ, true>(pl.N(g.r), pl.as, nt, pl.X(g.cur), pl.xs, mt, t.np / 32, ti, tj, acc, b0, b1, b2);
 
     // Lane (quad, col) holds rows 4 quad .. + 3 of column col of every 16 x 16 tile.  The results go through LDS and leave it
     // in short loops: read eight along a row, two tiles at a time, they are whole fragments; as they lie they are four
@@ -502,14 +495,14 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
     const int lane4 = (col + 16 * (quad >> 1)) * 8 + (quad & 1) * 4;     // this lane's place in a half fragment
     const int i0 = ti * (TI / 16) + (wave >> 1) * C::WI, j0 = tj * (TJ / 16) + (wave & 1) * C::WJ;
     // the A that c A^2 is added to: all of this wave's loads at once, as nothing else hides them
-    Quad4<P> old[ST == ST_POLY ? C::WI : 1][C::WJ];
+    Quad4 old[ST == ST_POLY ? C::WI : 1][C::WJ];
     if constexpr (ST == ST_POLY)
 #pragma unroll
         for (int i = 0; i < C::WI; ++i)
 #pragma unroll
             for (int j = 0; j < C::WJ; ++j) {
                 const int i16 = min(i0 + i, nt - 1), j16 = min(j0 + j, nt - 1);
-                old[i][j] = plane_load<P>(pl.N(g.r) + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4, pl.as);
+                old[i][j] = plane_load(pl.N(g.r) + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4, pl.as);
             }
     __syncthreads();                                                     // the operands in LDS are done with
     // a wave's own 16 x 16 tiles, QI rows of them at a time; 16 bytes after every 16 lanes and every tile starts 16 banks
@@ -528,7 +521,7 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
                 for (int r = 0; r < 4; ++r) {
                     v[r] *= unit;
                     if constexpr (ST == ST_POLY) {                       // A is symmetric: read as it lies, (column, row)
-                        v[r] = fmaf(NS_C, v[r], NS_B * plane_value<P>(old[c + q][j], r));
+                        v[r] = fmaf(NS_C, v[r], NS_B * plane_value(old[c + q][j], r));
                         if (i0 + c + q == j0 + j && 4 * quad + r == col) v[r] += NS_A;
                     }
                 }
@@ -550,11 +543,11 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
                         if (in) mu_put(a, t, j16 * 16 + col, i16 * 16 + 4 * quad, v, vec);
                     } else {
                         f16x4 h, l;
-                        split4<P>(v, h, l, g.plane);
+                        split4(v, h, l, g.plane);
                         _Float16* out = pl.N(g.out) + ((int64_t)j16 * (t.np >> 5) + (i16 >> 1)) * FRAG + (i16 & 1) * 256 + lane4;
                         if (in) {
                             *reinterpret_cast<f16x4*>(out) = h;
-                            if (P == 2) *reinterpret_cast<f16x4*>(out + pl.as) = l;
+                            *reinterpret_cast<f16x4*>(out + pl.as) = l;
                         }
                     }
                 }
@@ -590,7 +583,7 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
                         _Float16* out = (sym ? pl.N(g.out) : pl.X(g.cur ^ 1)) + ((int64_t)i16 * ((sym ? t.np : t.mp) >> 5) + (jp >> 1)) * FRAG + lane * 8;
                         if (in && (!sym || jp + (lane >> 5) < i16)) {    // on the diagonal the loop above stored the whole tile
                             *reinterpret_cast<f16x8*>(out) = h;
-                            if (P == 2) *reinterpret_cast<f16x8*>(out + (sym ? pl.as : pl.xs)) = l;
+                            *reinterpret_cast<f16x8*>(out + (sym ? pl.as : pl.xs)) = l;
                         }
                     }
                 }
@@ -604,16 +597,16 @@ __global__ __launch_bounds__(256) void mu_product_kernel(MuArgs a, MuStage g) {
 // wait in registers until everyone has read the operands they replace.  X is kept one way only: where k runs along its rows
 // the fragments are read with the transposing LDS read.  One launch for norm, five steps and update; the launches of the
 // general path cost 60 to 110 us whatever the size.  Measured, this way and that: 64 x 64 28 and 71 us, 64 x 192 37 and 80,
-// 128 x 192 69 and 88, 32 x 1000 73 and 103; bf16 128 x 192 47 and 77; the agent's five matrices 73 and 110.  Of 128 x 192's
-// step (25 k cycles) the products are half, bound by LDS reads; the rest is waiting for the slowest wave and storing.
+// 128 x 192 69 and 88, 32 x 1000 73 and 103; the agent's five matrices 73 and 110.  Of 128 x 192's step (25 k cycles) the
+// products are half, bound by LDS reads; the rest is waiting for the slowest wave and storing.
 constexpr int MU_SMALL_LDS = 160 * 1024;
-template <int P> struct MuSmall { static constexpr int NEXT = P == 2 ? 2 : 3, SYM = P == 2 ? 1 : 2; };      // most blocks a wave gets
+constexpr int MU_SMALL_NEXT = 2, MU_SMALL_SYM = 1;       // most blocks a wave gets
 
-template <int P> struct MuOperands { u32x4 r[P][2], c[P][2]; };
+struct MuOperands { u32x4 r[P][2], c[P][2]; };
 // k blocks one after the other, the next one's operands read while the current one is multiplied
-template <int P, typename Load, typename Multiply>
+template <typename Load, typename Multiply>
 __device__ __forceinline__ void mu_blocks(int K, const Load& load, const Multiply& multiply) {
-    MuOperands<P> x, y;
+    MuOperands x, y;
     load(x, 0);
 #pragma unroll 1
     for (int k = 0; k < K; k += 2) {
@@ -625,14 +618,13 @@ __device__ __forceinline__ void mu_blocks(int K, const Load& load, const Multipl
     }
 }
 
-static bool mu_is_small(int64_t rows, int64_t cols, int P) {
+static bool mu_is_small(int64_t rows, int64_t cols) {
     const int64_t n = round_up(rows < cols ? rows : cols, 32), m = round_up(rows < cols ? cols : rows, 32);
     const int64_t ni = n / 32, mi = m / 32;
-    return 2 * P * (n * m + n * n) <= MU_SMALL_LDS && ni * mi <= 16 * (P == 2 ? MuSmall<2>::NEXT : MuSmall<1>::NEXT)
-           && ni * (ni + 1) / 2 <= 16 * (P == 2 ? MuSmall<2>::SYM : MuSmall<1>::SYM);
+    return 2 * P * (n * m + n * n) <= MU_SMALL_LDS && ni * mi <= 16 * MU_SMALL_NEXT
+           && ni * (ni + 1) / 2 <= 16 * MU_SMALL_SYM;
 }
 
-template <int P>
 __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
     __shared__ __attribute__((aligned(16))) _Float16 lds[MU_SMALL_LDS / 2];
     const MuMat& t = a.mat[blockIdx.x];
@@ -699,7 +691,7 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
                 _Float16* o = X + ((row >> 4) * mb + (k >> 5)) * FRAG + (((row & 15) + 16 * ((k & 31) >> 3)) << 3) + (k & 7);
                 const _Float16 h = (_Float16)v;
                 o[0] = h;
-                if (P == 2) o[xs] = (_Float16)(v - (float)h);
+                o[xs] = (_Float16)(v - (float)h);
             }
         }
     __syncthreads();
@@ -733,16 +725,16 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
             const _Float16* src = st == ST_SYM ? X : A;
             const int64_t ps = st == ST_SYM ? xs : as;
             const int K = st == ST_SYM ? mb : nb;
-            f32x4 acc[MuSmall<P>::SYM][2][2];
+            f32x4 acc[MU_SMALL_SYM][2][2];
 #pragma unroll
-            for (int q = 0; q < MuSmall<P>::SYM; ++q) {
+            for (int q = 0; q < MU_SMALL_SYM; ++q) {
                 const int b = wave + 16 * q;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (b >= sym) continue;
                 int bi, bj;
                 block(b, bi, bj);
-                auto load = [&](MuOperands<P>& o, int k) {
+                auto load = [&](MuOperands& o, int k) {
 #pragma unroll
                     for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -751,13 +743,11 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
                             o.c[p][e] = frag(src + p * ps, 2 * bj + e, k, K);
                         }
                 };
-                mu_blocks<P>(K, load, [&](const MuOperands<P>& o) {
-                    if constexpr (P == 2) {
+                mu_blocks(K, load, [&](const MuOperands& o) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[1][e >> 1], o.c[0][e & 1], acc[q][e >> 1][e & 1]);
+                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[1][e >> 1], o.c[0][e & 1], acc[q][e >> 1][e & 1]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[0][e >> 1], o.c[1][e & 1], acc[q][e >> 1][e & 1]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[0][e >> 1], o.c[1][e & 1], acc[q][e >> 1][e & 1]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.r[0][e >> 1], o.c[0][e & 1], acc[q][e >> 1][e & 1]);
                 });
@@ -769,10 +759,10 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) v[x] *= unit;
                     if (st == ST_POLY) {
-                        const Quad4<P> o = plane_load<P>(A + frag_at(j16 * 16 + (lane & 15), i16 * 16 + (lane >> 4) * 4, np), as);
+                        const Quad4 o = plane_load(A + frag_at(j16 * 16 + (lane & 15), i16 * 16 + (lane >> 4) * 4, np), as);
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            v[x] = fmaf(NS_C, v[x], NS_B * plane_value<P>(o, x));
+                            v[x] = fmaf(NS_C, v[x], NS_B * plane_value(o, x));
                             if (i16 == j16 && (lane >> 4) * 4 + x == (lane & 15)) v[x] += NS_A;
                         }
                     }
@@ -780,7 +770,7 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
             }
             __syncthreads();                              // everyone has read A
 #pragma unroll
-            for (int q = 0; q < MuSmall<P>::SYM; ++q) {
+            for (int q = 0; q < MU_SMALL_SYM; ++q) {
                 const int b = wave + 16 * q;
                 if (b >= sym) continue;
                 int bi, bj;
@@ -791,16 +781,16 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
                     if (j16 > i16) continue;
                     const float v[4] = {acc[q][e >> 1][e & 1][0], acc[q][e >> 1][e & 1][1], acc[q][e >> 1][e & 1][2], acc[q][e >> 1][e & 1][3]};
                     f16x4 h, l;
-                    split4<P>(v, h, l);
+                    split4(v, h, l);
                     _Float16* o = A + frag_at(j16 * 16 + (lane & 15), i16 * 16 + (lane >> 4) * 4, np);
                     *reinterpret_cast<f16x4*>(o) = h;
-                    if (P == 2) *reinterpret_cast<f16x4*>(o + as) = l;
+                    *reinterpret_cast<f16x4*>(o + as) = l;
                     if (i16 != j16) {
                         o = A + frag_at(i16 * 16 + (lane >> 4) * 4, j16 * 16 + (lane & 15), np);
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {     // rows 8 halves apart
                             o[x * 8] = h[x];
-                            if (P == 2) o[x * 8 + as] = l[x];
+                            o[x * 8 + as] = l[x];
                         }
                     }
                 }
@@ -808,14 +798,14 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
             __syncthreads();
         }
         // X <- B X; the instruction's rows are X's columns, so that a lane ends with four neighbours of one row
-        f32x4 acc[MuSmall<P>::NEXT][2][2];
+        f32x4 acc[MU_SMALL_NEXT][2][2];
 #pragma unroll
-        for (int q = 0; q < MuSmall<P>::NEXT; ++q) {
+        for (int q = 0; q < MU_SMALL_NEXT; ++q) {
             const int b = wave + 16 * q, bi = b % nb, bj = b / nb;
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (b >= full) continue;
-            auto load = [&](MuOperands<P>& o, int k) {
+            auto load = [&](MuOperands& o, int k) {
 #pragma unroll
                 for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -824,13 +814,11 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
                         o.c[p][e] = frag_tr(X + p * xs, 2 * bj + e, k);
                     }
             };
-            mu_blocks<P>(nb, load, [&](const MuOperands<P>& o) {
-                if constexpr (P == 2) {
+            mu_blocks(nb, load, [&](const MuOperands& o) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[0][e & 1], o.r[1][e >> 1], acc[q][e >> 1][e & 1]);
+                for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[0][e & 1], o.r[1][e >> 1], acc[q][e >> 1][e & 1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[1][e & 1], o.r[0][e >> 1], acc[q][e >> 1][e & 1]);
-                }
+                for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[1][e & 1], o.r[0][e >> 1], acc[q][e >> 1][e & 1]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[q][e >> 1][e & 1] = mfma_h(o.c[0][e & 1], o.r[0][e >> 1], acc[q][e >> 1][e & 1]);
             });
@@ -838,7 +826,7 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
         __syncthreads();                                  // everyone has read X
         const bool vec = (t.ldo & 3) == 0 && (t.cols & 3) == 0 && ((uintptr_t)t.out & (t.mom || a.otype == MU_F32 ? 15 : 7)) == 0;
 #pragma unroll
-        for (int q = 0; q < MuSmall<P>::NEXT; ++q) {
+        for (int q = 0; q < MU_SMALL_NEXT; ++q) {
             const int b = wave + 16 * q, bi = b % nb, bj = b / nb;
             if (b >= full) continue;
 #pragma unroll
@@ -849,10 +837,10 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
                 for (int x = 0; x < 4; ++x) v[x] = acc[q][e >> 1][e & 1][x] * (UNPLANE * UNPLANE * sc);
                 if (it < 4) {
                     f16x4 h, l;
-                    split4<P>(v, h, l);
+                    split4(v, h, l);
                     _Float16* o = X + frag_at(gi, gj, mp);
                     *reinterpret_cast<f16x4*>(o) = h;
-                    if (P == 2) *reinterpret_cast<f16x4*>(o + xs) = l;
+                    *reinterpret_cast<f16x4*>(o + xs) = l;
                 } else if (!tr) mu_put(a, t, gi, gj, v, vec);
                 else
 #pragma unroll
@@ -866,14 +854,14 @@ __global__ __launch_bounds__(1024) void mu_small_kernel(MuArgs a) {
 // ---- host ------------------------------------------------------------------------------------------------------------------
 constexpr int MU_PAD = 64;          // sides are padded to this; larger tiles repeat the last rows and drop them
 
-static int64_t mu_matrix_bytes(int64_t rows, int64_t cols, int P) {
+static int64_t mu_matrix_bytes(int64_t rows, int64_t cols) {
     const int64_t n = rows < cols ? rows : cols, m = rows < cols ? cols : rows;
     const int64_t np = round_up(n, MU_PAD), mp = round_up(m, MU_PAD);
     return round_up(2 * P * (2 * np * mp + 4 * np * np), 256) + MU_PARTS * 8;
 }
-static int64_t mu_group_bytes(const mctsq_muon_matrix* mats, int count, int P) {
+static int64_t mu_group_bytes(const mctsq_muon_matrix* mats, int count) {
     int64_t o = 0;
-    for (int i = 0; i < count; ++i) o += mu_matrix_bytes(mats[i].rows, mats[i].cols, P);
+    for (int i = 0; i < count; ++i) o += mu_matrix_bytes(mats[i].rows, mats[i].cols);
     return o;
 }
 static int mu_check_shapes(const mctsq_muon_matrix* mats, int64_t count) {
@@ -884,10 +872,10 @@ static int mu_check_shapes(const mctsq_muon_matrix* mats, int64_t count) {
                     (long long)mats[i].cols);
     return 0;
 }
-static int64_t mu_bytes(const mctsq_muon_matrix* mats, int64_t count, int P) {
+static int64_t mu_bytes(const mctsq_muon_matrix* mats, int64_t count) {
     int64_t need = 0;                                    // the groups run one after the other in the same space
     for (int64_t g = 0; g < count; g += MU_GROUP) {
-        const int64_t b = mu_group_bytes(mats + g, (int)(count - g < MU_GROUP ? count - g : MU_GROUP), P);
+        const int64_t b = mu_group_bytes(mats + g, (int)(count - g < MU_GROUP ? count - g : MU_GROUP));
         need = b > need ? b : need;
     }
     return need < 256 ? 256 : need;
@@ -910,27 +898,26 @@ static double mu_stage(MuArgs& a, bool sym, bool gram, double step, double over,
     return work / tiles * step * load + over * ((load + share - 1) / share);
 }
 // Launches the stage on the tiles that the estimate prefers, or only estimates it.
-template <int P, int ST>
+template <int ST>
 static double mu_product(MuArgs& a, const MuStage& g, hipStream_t st, bool launch) {
     constexpr bool sym = ST == ST_SYM || ST == ST_POLY;
     const bool gram = ST == ST_SYM && g.r < 0;
-    // fp32: 256 x 128 tiles 0.87 us a k block (0.73 at the matrix pipe's rate) and 23 a tile, 128 x 128 0.50 and 15, 64 x 64
-    // 0.20 and 8 with three to a CU; bf16: 0.33 / 15, 0.19 / 8, 0.10 / 5
-    static constexpr double STEP[2][3] = {{0.33, 0.19, 0.10}, {0.87, 0.50, 0.20}}, OVER[2][3] = {{15, 8, 5}, {23, 15, 8}};
+    // 256 x 128 tiles 0.87 us a k block (0.73 at the matrix pipe's rate) and 23 a tile, 128 x 128 0.50 and 15, 64 x 64 0.20 and
+    // 8 with three to a CU
     int tiles;
-    const double t256 = mu_stage<256, 128>(a, sym, gram, STEP[P - 1][0], OVER[P - 1][0], 1, tiles);
-    const double t128 = mu_stage<128, 128>(a, sym, gram, STEP[P - 1][1], OVER[P - 1][1], P == 2 ? 1 : 2, tiles);
-    const double t64 = mu_stage<64, 64>(a, sym, gram, STEP[P - 1][2], OVER[P - 1][2], 3, tiles);      // a.first as for 64 x 64
+    const double t256 = mu_stage<256, 128>(a, sym, gram, 0.87, 23, 1, tiles);
+    const double t128 = mu_stage<128, 128>(a, sym, gram, 0.50, 15, 1, tiles);
+    const double t64 = mu_stage<64, 64>(a, sym, gram, 0.20, 8, 3, tiles);              // a.first as for 64 x 64
     const double best = std::min(t64, std::min(t128, t256));
     if (!launch) return best;
     if (t64 == best) {
-        hipLaunchKernelGGL((mu_product_kernel<P, 64, 64, ST>), dim3(tiles), dim3(256), 0, st, a, g);
+        hipLaunchKernelGGL((mu_product_kernel<64, 64, ST>), dim3(tiles), dim3(256), 0, st, a, g);
     } else if (t128 == best) {
         mu_stage<128, 128>(a, sym, gram, 0, 0, 1, tiles);
-        hipLaunchKernelGGL((mu_product_kernel<P, 128, 128, ST>), dim3(tiles), dim3(256), 0, st, a, g);
+        hipLaunchKernelGGL((mu_product_kernel<128, 128, ST>), dim3(tiles), dim3(256), 0, st, a, g);
     } else {
         mu_stage<256, 128>(a, sym, gram, 0, 0, 1, tiles);
-        hipLaunchKernelGGL((mu_product_kernel<P, 256, 128, ST>), dim3(tiles), dim3(256), 0, st, a, g);
+        hipLaunchKernelGGL((mu_product_kernel<256, 128, ST>), dim3(tiles), dim3(256), 0, st, a, g);
     }
     return best;
 }
@@ -939,35 +926,33 @@ static double mu_product(MuArgs& a, const MuStage& g, hipStream_t st, bool launc
 // step before it, A' = Q A Q with Q = a + b A + c A^2, as X' = Q X; so the chain needs X only at its ends:
 //   A = X X^T;  per step Q = a + b A + c A^2, N <- Q N, A <- (Q A) Q;  X <- N X
 // 3 n^2 m + (4 chain - 3) n^3 in place of chain (3 n^2 m + n^3).  N's values reach 3.4445^chain, its planes 2^(16 - 2 chain).
-template <int P>
 static double mu_steps(MuArgs& a, int chain, int cur, bool scaled, bool last, hipStream_t st, bool launch) {
     const float u2 = UNPLANE * UNPLANE;
     // n x n matrices: 0 A, 1 .. 3 Q, N and Q A in turn
-    double t = mu_product<P, ST_SYM>(a, MuStage{-1, -1, 0, cur, scaled, u2, PLANE}, st, launch);
+    double t = mu_product<ST_SYM>(a, MuStage{-1, -1, 0, cur, scaled, u2, PLANE}, st, launch);
     int q = 1, n = 1;
     float np = PLANE;
-    t += mu_product<P, ST_POLY>(a, MuStage{0, 0, q, cur, 0, u2, PLANE}, st, launch);
+    t += mu_product<ST_POLY>(a, MuStage{0, 0, q, cur, 0, u2, PLANE}, st, launch);
     for (int k = 1; k < chain; ++k) {
         const int w = 6 - q - n == 4 ? 2 : 6 - q - n;                        // the one that is neither (any of two where q = n)
-        t += mu_product<P, ST_SYM>(a, MuStage{q, 0, w, cur, 0, u2, PLANE}, st, launch);             // Q A
-        t += mu_product<P, ST_SYM>(a, MuStage{w, q, 0, cur, 0, u2, PLANE}, st, launch);             // (Q A) Q
+        t += mu_product<ST_SYM>(a, MuStage{q, 0, w, cur, 0, u2, PLANE}, st, launch);             // Q A
+        t += mu_product<ST_SYM>(a, MuStage{w, q, 0, cur, 0, u2, PLANE}, st, launch);             // (Q A) Q
         q = w;
-        t += mu_product<P, ST_POLY>(a, MuStage{0, 0, q, cur, 0, u2, PLANE}, st, launch);
+        t += mu_product<ST_POLY>(a, MuStage{0, 0, q, cur, 0, u2, PLANE}, st, launch);
         const int o = 6 - q - n;
-        t += mu_product<P, ST_SYM>(a, MuStage{q, n, o, cur, 0, UNPLANE / np, np / 4}, st, launch);  // N
+        t += mu_product<ST_SYM>(a, MuStage{q, n, o, cur, 0, UNPLANE / np, np / 4}, st, launch);  // N
         n = o;
         np /= 4;
     }
     const MuStage end{n, -1, -1, cur, scaled, UNPLANE / np, PLANE};
-    return t + (last ? mu_product<P, ST_LAST>(a, end, st, launch) : mu_product<P, ST_NEXT>(a, end, st, launch));
+    return t + (last ? mu_product<ST_LAST>(a, end, st, launch) : mu_product<ST_NEXT>(a, end, st, launch));
 }
 
-template <int P>
 static void mu_launch(MuArgs& a, hipStream_t st) {
     bool small = true;
-    for (int i = 0; i < a.count; ++i) small = small && mu_is_small(a.mat[i].rows, a.mat[i].cols, P);
+    for (int i = 0; i < a.count; ++i) small = small && mu_is_small(a.mat[i].rows, a.mat[i].cols);
     if (small) {
-        hipLaunchKernelGGL(mu_small_kernel<P>, dim3(a.count), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL(mu_small_kernel, dim3(a.count), dim3(1024), 0, st, a);
         return;
     }
     hipLaunchKernelGGL(mu_norm_kernel, dim3(MU_PARTS, a.count), dim3(256), 0, st, a);
@@ -976,16 +961,15 @@ static void mu_launch(MuArgs& a, hipStream_t st) {
         a.first[i] = i < a.count ? blk : INT_MAX;
         if (i < a.count) blk += (a.mat[i].np / 64) * (a.mat[i].mp / 64);
     }
-    hipLaunchKernelGGL(mu_planes_kernel<P>, dim3(blk), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(mu_planes_kernel, dim3(blk), dim3(256), 0, st, a);
     // One step at a time; or two, one, two at once, or two and three, where the products that saves are worth more than the
     // launches it adds (large matrices, the wider the more).  Errors against 64 bits, fp32, worst of five shapes and three
     // spectra (elementary fp32 operations 5.6e-6 and 1.3e-4 where four directions carry all but 1e-3): one by one 3.6e-6
     // and 1.5e-4, two-one-two 3.1e-6 and 9.5e-5, two-three 4.4e-6 and 9.8e-5, the 4.4e-6 at 1000 x 1500, hence 2 n <= m.
-    // bf16 (rounding alone 1.7e-3): 2.2e-3 and 3.9e-2, 2.2e-3 and 9.9e-3, 4.2e-3 and 6.1e-2: never two-three.
     static constexpr int PLAN[3][6] = {{1, 1, 1, 1, 1, 0}, {2, 1, 2, 0, 0, 0}, {2, 3, 0, 0, 0, 0}};
     double one = 0.0, cost[4];
-    for (int c = 1; c <= 3; ++c) cost[c] = mu_steps<P>(a, c, 0, false, false, st, false);
-    bool wide = P == 2;
+    for (int c = 1; c <= 3; ++c) cost[c] = mu_steps(a, c, 0, false, false, st, false);
+    bool wide = true;
     for (int i = 0; i < a.count; ++i) wide = wide && a.mat[i].m >= 2 * a.mat[i].n;
     int plan = 0;
     for (int i = 0; i < (wide ? 3 : 2); ++i) {
@@ -994,10 +978,10 @@ static void mu_launch(MuArgs& a, hipStream_t st) {
         if (i == 0 || t < 0.97 * one) { one = t; plan = i; }
     }
     for (int c = 0, cur = 0; PLAN[plan][c]; ++c, cur ^= 1)
-        mu_steps<P>(a, PLAN[plan][c], cur, c == 0, PLAN[plan][c + 1] == 0, st, true);
+        mu_steps(a, PLAN[plan][c], cur, c == 0, PLAN[plan][c + 1] == 0, st, true);
 }
 
-static int mu_run(const mctsq_muon_matrix* mats, int64_t count, int P, MuArgs& a, double lr, int adjust, char* ws, hipStream_t st) {
+static int mu_run(const mctsq_muon_matrix* mats, int64_t count, MuArgs& a, double lr, int adjust, char* ws, hipStream_t st) {
     for (int64_t g = 0; g < count; g += MU_GROUP) {
         const int c = (int)(count - g < MU_GROUP ? count - g : MU_GROUP);
         int64_t o = 0, blk = 0;
@@ -1020,13 +1004,12 @@ static int mu_run(const mctsq_muon_matrix* mats, int64_t count, int P, MuArgs& a
             t.lrs = (float)(lr * (adjust == MCTSQ_MUON_SPECTRAL ? sqrt(r > k ? r / k : 1.0)
                                   : adjust == MCTSQ_MUON_RMS ? 0.2 * sqrt(r > k ? r : k) : 1.0));
             t.ws = (_Float16*)(ws + o);
-            o += mu_matrix_bytes(s.rows, s.cols, P);
+            o += mu_matrix_bytes(s.rows, s.cols);
             t.part = (double*)(ws + o) - MU_PARTS;
             blk += (int64_t)(t.np / 64) * (t.mp / 64);
         }
         MCTSQ_CHECK(blk < ((int64_t)1 << 31), "the matrices of one group are too large");
-        if (P == 2) mu_launch<2>(a, st);
-        else mu_launch<1>(a, st);
+        mu_launch(a, st);
         MCTSQ_HIP(hipGetLastError());
     }
     return 0;
@@ -1039,7 +1022,7 @@ using namespace mctsq;
 extern "C" int64_t mctsq_orthogonalize_workspace_bytes(const mctsq_muon_matrix* mats, int64_t count, int dtype) {
     if (int rc = mu_check_shapes(mats, count)) return rc;
     MCTSQ_CHECK(dtype == MU_F32 || dtype == MU_BF16, "dtype must be 0 (fp32) or 1 (bf16)");
-    return mu_bytes(mats, count, dtype == MU_F32 ? 2 : 1);
+    return mu_bytes(mats, count);
 }
 extern "C" int mctsq_orthogonalize(const mctsq_muon_matrix* mats, int64_t count, int dtype, double eps, void* d_ws,
                                    int64_t ws_bytes, void* stream) {
@@ -1057,12 +1040,12 @@ extern "C" int mctsq_orthogonalize(const mctsq_muon_matrix* mats, int64_t count,
     }
     MuArgs a{};
     a.xtype = a.otype = dtype; a.eps = eps;
-    return mu_run(mats, count, dtype == MU_F32 ? 2 : 1, a, 1.0, MCTSQ_MUON_NONE, (char*)d_ws, (hipStream_t)stream);
+    return mu_run(mats, count, a, 1.0, MCTSQ_MUON_NONE, (char*)d_ws, (hipStream_t)stream);
 }
 
 extern "C" int64_t mctsq_muon_workspace_bytes(const mctsq_muon_matrix* mats, int64_t count) {
     if (int rc = mu_check_shapes(mats, count)) return rc;
-    return mu_bytes(mats, count, 2);
+    return mu_bytes(mats, count);
 }
 extern "C" int mctsq_muon_step(const mctsq_muon_matrix* mats, int64_t count, int grad_dtype, double lr, double momentum,
                                int nesterov, double weight_decay, double eps, int adjust, void* d_ws, int64_t ws_bytes,
@@ -1086,5 +1069,5 @@ extern "C" int mctsq_muon_step(const mctsq_muon_matrix* mats, int64_t count, int
     MuArgs a{};
     a.xtype = grad_dtype; a.otype = MU_F32; a.eps = eps;
     a.mu = (float)momentum; a.nesterov = nesterov; a.decay = (float)(1.0 - lr * weight_decay);
-    return mu_run(mats, count, 2, a, lr, adjust, (char*)d_ws, (hipStream_t)stream);
+    return mu_run(mats, count, a, lr, adjust, (char*)d_ws, (hipStream_t)stream);
 }

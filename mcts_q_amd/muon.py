@@ -2,9 +2,8 @@
 (`orthogonalize`) and the optimizer whose step it is (`DeviceMuon`).
 
 The iteration replaces a matrix by roughly the nearest semi-orthogonal one: X = x / |x|_F, then five times
-X <- 3.4445 X + (-4.7750 A + 2.0315 A^2) X with A = X X^T.  fp32 matrices are evaluated to fp32 accuracy, bf16 matrices
-with operands of 11 bits (directions weaker than 2^-11 of the strongest are lost).  Everything is enqueued on the current
-stream of the tensors' device; nothing synchronises."""
+X <- 3.4445 X + (-4.7750 A + 2.0315 A^2) X with A = X X^T, evaluated to fp32 accuracy; the result of a bf16 matrix is rounded
+once, at the end.  Everything is enqueued on the current stream of the tensors' device; nothing synchronises."""
 from __future__ import annotations
 
 from bisect import bisect_left
