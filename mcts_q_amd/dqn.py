@@ -315,35 +315,78 @@ class _RingView:
 
 
 class _AdamFacade:
-    """`DQNModel.optimizer` stand-in exposing torch.optim.Adam's state_dict layout (dqn_per.py:486, 503)."""
+    """`DQNModel.optimizer` stand-in exposing torch.optim.Adam's state_dict layout (dqn_per.py:486, 503).
+
+    A Muon learner's state has a second parameter group, marked "optimizer": "muon", and its matrices' state is
+    {"step", "momentum_buffer"}: torch's Adam refuses such a file, and the two optimizers here refuse each other's."""
 
     def __init__(self, learner: DeviceLearner, lr: float):
         self.learner, self.lr = learner, lr
 
+    def _muon_indices(self):
+        keys = set(self.learner.muon_keys())
+        return [i for i, (k, _) in enumerate(self.learner.spec.param_keys()) if k in keys]
+
     def state_dict(self):
         L = self.learner
         m, v = L.policy.views(L.exp_avg), L.policy.views(L.exp_avg_sq)
+        by_muon = self._muon_indices() if L.optimizer == "muon" else []
         state = {}
         if L.step_count > 0:
             for i, k in enumerate(m):
-                state[i] = {"step": torch.tensor(float(L.step_count)), "exp_avg": m[k].detach().cpu().clone(),
-                            "exp_avg_sq": v[k].detach().cpu().clone()}
+                state[i] = {"step": torch.tensor(float(L.step_count))}
+                if i in by_muon:
+                    state[i]["momentum_buffer"] = m[k].detach().cpu().clone()
+                else:
+                    state[i].update(exp_avg=m[k].detach().cpu().clone(), exp_avg_sq=v[k].detach().cpu().clone())
         group = {"lr": self.lr, "betas": tuple(L.betas), "eps": L.eps, "weight_decay": 0, "amsgrad": False,
                  "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
-                 "decoupled_weight_decay": False, "params": list(range(len(m)))}
-        return {"state": state, "param_groups": [group]}
+                 "decoupled_weight_decay": False, "params": [i for i in range(len(m)) if i not in by_muon]}
+        groups = [group]
+        if L.optimizer == "muon":
+            groups.append({"optimizer": "muon", "lr": L.muon.lr, "momentum": L.muon.momentum, "nesterov": L.muon.nesterov,
+                           "weight_decay": L.muon.weight_decay, "eps": L.muon.eps, "adjust": L.muon.adjust,
+                           "params": by_muon})
+        return {"state": state, "param_groups": groups}
+
+    def check_state_dict(self, sd):
+        """ValueError where the state is the other optimizer's.  A single group without the mark is Adam's, or Muon's
+        momentum written as exp_avg with exp_avg_sq 0, told by its values: m^2 <= 53 v in Adam, so its m is below 1e-16
+        where v rounded to 0."""
+        muon = self.learner.optimizer == "muon"
+        marked = any(g.get("optimizer") == "muon" for g in sd["param_groups"])
+        theirs = [sd["state"][i] for i in self._muon_indices() if i in sd["state"]]
+        if not marked:
+            momentum = [not s["exp_avg_sq"].any() and float(s["exp_avg"].abs().max()) > 1e-16 for s in theirs]
+            adam = any(bool(s["exp_avg_sq"].any()) for s in theirs)
+        if muon and not marked and adam:
+            raise ValueError("the optimizer state is Adam's, this model's optimizer is Muon: build it with optimizer='adam', "
+                             "or load the networks alone")
+        if not muon and (marked or any(momentum)):
+            raise ValueError("the optimizer state is Muon's, this model's optimizer is Adam: build it with optimizer='muon', "
+                             "or load the networks alone")
+        if marked and sd["param_groups"][1]["params"] != self._muon_indices():
+            raise ValueError("the optimizer state's Muon matrices are not this network's")
 
     def load_state_dict(self, sd):
+        self.check_state_dict(sd)
         L = self.learner
         m, v = L.policy.views(L.exp_avg), L.policy.views(L.exp_avg_sq)
         L.exp_avg.zero_(); L.exp_avg_sq.zero_()
         steps = [int(float(s["step"])) for s in sd["state"].values()]
         L.step_count = max(steps) if steps else 0
         for i, k in enumerate(m):
-            if i in sd["state"]:
-                m[k].copy_(sd["state"][i]["exp_avg"]); v[k].copy_(sd["state"][i]["exp_avg_sq"])
+            s = sd["state"].get(i, {})
+            if "momentum_buffer" in s:
+                m[k].copy_(s["momentum_buffer"])
+            elif s:
+                m[k].copy_(s["exp_avg"]); v[k].copy_(s["exp_avg_sq"])
         g = sd["param_groups"][0]
         self.lr = L.lr = float(g["lr"]); L.betas = tuple(g["betas"]); L.eps = float(g["eps"])
+        if len(sd["param_groups"]) > 1:
+            g = sd["param_groups"][1]
+            L.muon.lr, L.muon.momentum, L.muon.nesterov = float(g["lr"]), float(g["momentum"]), bool(g["nesterov"])
+            L.muon.weight_decay, L.muon.eps, L.muon.adjust = float(g["weight_decay"]), float(g["eps"]), g["adjust"]
 
     def zero_grad(self):
         self.learner.grad.zero_()
@@ -429,6 +472,7 @@ class DQNModel:
                       [type(np.dtype(t)) for t in (np.float32, np.float64, np.int64, np.int32, np.bool_)]
             with torch.serialization.safe_globals(allowed):
                 ckpt = torch.load(filepath, map_location="cpu", weights_only=True)
+        self.optimizer.check_state_dict(ckpt["optimizer_state_dict"])       # before anything is changed
         self.policy_net.load_state_dict(ckpt["policy_net_state_dict"])
         self.target_net.load_state_dict(ckpt["target_net_state_dict"])
         self.optimizer.load_state_dict(ckpt["optimizer_state_dict"])
