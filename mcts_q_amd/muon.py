@@ -7,10 +7,12 @@ once, at the end.  Everything is enqueued on the current stream of the tensors' 
 from __future__ import annotations
 
 from bisect import bisect_left
+from itertools import accumulate
 
 import torch
 
 from ._lib import MctsqError, MuonMatrix, lib, on_device, ptr, stream_ptr
+from ._memory import overlaps_itself, share_memory, span
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 _ADJUST = {"none": 0, "spectral": 1, "rms": 2}
@@ -41,14 +43,17 @@ def _slices(t):
     return [t.data_ptr() + i * step for i in range(t.shape[0])]
 
 
-def _span(t):
-    """[first, last) byte addresses a strided tensor touches."""
-    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())))
-
-
-def _rows_overlap(t):
-    """Whether the rows of a stack share memory with each other."""
-    return t.dim() == 3 and t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * _ld(t) + t.shape[2]
+def _sharing_pair(tensors):
+    """Indices of two tensors that share memory, or None."""
+    spans = [span(t) for t in tensors]
+    reached = []                                             # those whose end lies past the current start
+    for i in sorted(range(len(tensors)), key=spans.__getitem__):
+        reached = [j for j in reached if spans[j][1] > spans[i][0]]
+        for j in reached:
+            if share_memory(tensors[i], tensors[j]):
+                return min(i, j), max(i, j)
+        reached.append(i)
+    return None
 
 
 def orthogonalize(x, eps=1e-7, out=None):
@@ -63,12 +68,10 @@ def orthogonalize(x, eps=1e-7, out=None):
                          f"with strides {x.stride()}")
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not _is_matrix(out) or _rows_overlap(out):
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not _is_matrix(out) or overlaps_itself(out):
         raise ValueError(f"out: expected {tuple(x.shape)} {x.dtype} on {x.device} with contiguous rows that do not overlap")
-    elif not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
-        (a0, a1), (b0, b1) = _span(x), _span(out)
-        if a0 < b1 and b0 < a1:
-            raise ValueError("out: must be x itself or share no memory with it")
+    elif not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) and share_memory(x, out):
+        raise ValueError("out: must be x itself or share no memory with it")
     r, c = x.shape[-2:]
     src, dst = _slices(x), _slices(out)
     lx, lo = _ld(x), _ld(out)
@@ -101,15 +104,12 @@ class DeviceMuon:
         for i, p in enumerate(params):
             if not isinstance(p, torch.Tensor) or not p.is_cuda:
                 raise MctsqError("DeviceMuon needs parameters on the GPU: the HIP path has no CPU fallback")
-            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != params[0].device or _rows_overlap(p):
+            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != params[0].device or overlaps_itself(p):
                 raise ValueError(f"params[{i}]: expected fp32 [rows, cols] or [count, rows, cols] with contiguous rows on "
                                  f"{params[0].device}, got {tuple(p.shape)} {p.dtype} with strides {p.stride()} on {p.device}")
-        spans = sorted((*_span(p), i) for i, p in enumerate(params) if p.is_contiguous())
-        for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
-            if start < end:
-                raise ValueError(f"params[{i}] and params[{j}] share memory")
-        if len({p.data_ptr() for p in params}) < len(params):
-            raise ValueError("params: the same matrix twice")
+        pair = _sharing_pair(params)
+        if pair:
+            raise ValueError("params[%d] and params[%d] share memory" % pair)
         if adjust not in _ADJUST:
             raise ValueError(f"adjust: expected one of {sorted(_ADJUST)}, got {adjust!r}")
         if not 0.0 <= momentum < 1.0:
@@ -123,12 +123,12 @@ class DeviceMuon:
             if m.shape != p.shape or m.dtype != torch.float32 or m.device != p.device or not m.is_contiguous():
                 raise ValueError(f"momentum_buffers[{i}]: expected contiguous fp32 {tuple(p.shape)} on {p.device}")
         self.momentum_buffers = list(momentum_buffers)
-        # what a step writes, in the order of memory (of strided parameters their bounds may interleave: the starts alone)
-        self._starts = {p.data_ptr() for p in params}
-        written = sorted(_span(t) for t in self.momentum_buffers + [p for p in params if p.is_contiguous()])
-        if any(b0 < a1 for (_, a1), (b0, _) in zip(written, written[1:])):
+        if _sharing_pair(params + self.momentum_buffers):
             raise ValueError("momentum_buffers: must share no memory with each other or the parameters")
-        self._first, self._last = [a for a, _ in written], [b for _, b in written]
+        # what a step writes, in the order of memory: starts, and how far everything up to there reaches
+        self._written = sorted(params + self.momentum_buffers, key=span)
+        self._first = [span(t)[0] for t in self._written]
+        self._reach = list(accumulate((span(t)[1] for t in self._written), max))
         mats, self._spans = [], []
         for p, m in zip(params, self.momentum_buffers):
             ps, ms = _slices(p), _slices(m)
@@ -151,9 +151,9 @@ class DeviceMuon:
             if g.shape != p.shape or g.dtype != dt or g.device != self.device or not _is_matrix(g):
                 raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {dt} on {self.device} with contiguous rows, got "
                                  f"{tuple(g.shape)} {g.dtype} with strides {g.stride()} on {g.device}")
-            a, b = _span(g)
-            k = bisect_left(self._first, b)                  # the last written range that starts before the gradient's end
-            if (k and self._last[k - 1] > a) or a in self._starts:
+            a, b = span(g)
+            k = bisect_left(self._first, b)                  # what starts before the gradient's end; most reaches not as far
+            if k and self._reach[k - 1] > a and any(share_memory(g, t) for t in self._written[:k]):
                 raise ValueError(f"grads[{i}]: must share no memory with the parameters or the momentum")
             ld = _ld(g)
             for j, q in enumerate(_slices(g)):

@@ -19,6 +19,7 @@ import functools
 import torch
 
 from ._lib import MctsqError, lib, on_device, ptr, stream_ptr
+from ._memory import share_memory
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -62,12 +63,6 @@ def _vec(name, t, shape, device):
                          f"{t.device}")
 
 
-def _span(t):
-    """[first, last) byte addresses a strided tensor touches."""
-    end = t.data_ptr() + t.element_size() * (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())))
-    return t.data_ptr(), end
-
-
 def _grad_out(logits, out):
     if out is None:
         return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -75,10 +70,8 @@ def _grad_out(logits, out):
             or (out.shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError(f"out: expected {tuple(logits.shape)} {logits.dtype} on {logits.device} with contiguous rows, got "
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
-    if out.numel() and not (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()):
-        (a0, a1), (b0, b1) = _span(logits), _span(out)
-        if a0 < b1 and b0 < a1:
-            raise ValueError("out: must be the logits themselves or share no memory with them")
+    if not (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()) and share_memory(logits, out):
+        raise ValueError("out: must be the logits themselves or share no memory with them")
     return out
 
 
