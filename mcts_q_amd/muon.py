@@ -94,60 +94,85 @@ class DeviceMuon:
     [rows, cols] or a stack [count, rows, cols] of matrices, rows contiguous.  Gradients are fp32 or bf16, all of one type.
     They share no memory with the parameters or the state: `momentum_buffers` (fp32, contiguous, one per parameter).  The
     workspace is kept, so steps of one instance belong on one stream at a time (two graphs captured from one instance must
-    not run at once), and an instance has to live as long as the graphs captured from it."""
+    not run at once), and an instance has to live as long as the graphs captured from it.  Parameters that move between
+    steps (`p.data = ...`) are followed; a captured graph keeps the addresses it was captured with."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, eps=1e-7, adjust="spectral",
                  momentum_buffers=None):
         params = list(params)
         if not params:
             raise ValueError("params: empty")
-        for i, p in enumerate(params):
-            if not isinstance(p, torch.Tensor) or not p.is_cuda:
-                raise MctsqError("DeviceMuon needs parameters on the GPU: the HIP path has no CPU fallback")
-            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != params[0].device or overlaps_itself(p):
-                raise ValueError(f"params[{i}]: expected fp32 [rows, cols] or [count, rows, cols] with contiguous rows on "
-                                 f"{params[0].device}, got {tuple(p.shape)} {p.dtype} with strides {p.stride()} on {p.device}")
-        pair = _sharing_pair(params)
-        if pair:
-            raise ValueError("params[%d] and params[%d] share memory" % pair)
         if adjust not in _ADJUST:
             raise ValueError(f"adjust: expected one of {sorted(_ADJUST)}, got {adjust!r}")
         if not 0.0 <= momentum < 1.0:
             raise ValueError(f"momentum must lie in [0, 1), got {momentum}")
+        self._check_params(params, getattr(params[0], "device", None))
         self.params, self.device = params, params[0].device
         self.lr, self.momentum, self.nesterov = float(lr), float(momentum), bool(nesterov)
         self.weight_decay, self.eps, self.adjust = float(weight_decay), float(eps), adjust
         if momentum_buffers is None:
             momentum_buffers = [torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in params]
-        for i, (p, m) in enumerate(zip(params, momentum_buffers, strict=True)):
+        self.momentum_buffers = list(momentum_buffers)
+        self._lay_out()
+        with on_device(self.device):
+            self._ws_bytes = lib.check(lib.mctsq_muon_workspace_bytes(self._mats, len(self._mats)))
+            self._ws = _aligned(self._ws_bytes, self.device)
+            self._ws_stream = stream_ptr(self.device)
+
+    @staticmethod
+    def _check_params(params, device):
+        for i, p in enumerate(params):
+            if not isinstance(p, torch.Tensor) or not p.is_cuda:
+                raise MctsqError("DeviceMuon needs parameters on the GPU: the HIP path has no CPU fallback")
+            if p.dtype != torch.float32 or not _is_matrix(p) or p.device != device or overlaps_itself(p):
+                raise ValueError(f"params[{i}]: expected fp32 [rows, cols] or [count, rows, cols] with contiguous rows on "
+                                 f"{device}, got {tuple(p.shape)} {p.dtype} with strides {p.stride()} on {p.device}")
+        pair = _sharing_pair(params)
+        if pair:
+            raise ValueError("params[%d] and params[%d] share memory" % pair)
+
+    def _places(self):
+        """Where parameters and momentum lie; `p.data = ...` (Module.to and the like) moves them."""
+        return [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in (*self.params, *self.momentum_buffers)]
+
+    def _lay_out(self):
+        """The matrices' descriptions and the ranges a step writes, of the tensors as they are now."""
+        params = self.params
+        for i, (p, m) in enumerate(zip(params, self.momentum_buffers, strict=True)):
             if m.shape != p.shape or m.dtype != torch.float32 or m.device != p.device or not m.is_contiguous():
                 raise ValueError(f"momentum_buffers[{i}]: expected contiguous fp32 {tuple(p.shape)} on {p.device}")
-        self.momentum_buffers = list(momentum_buffers)
         if _sharing_pair(params + self.momentum_buffers):
             raise ValueError("momentum_buffers: must share no memory with each other or the parameters")
         # what a step writes, in the order of memory: starts, and how far everything up to there reaches
         self._written = sorted(params + self.momentum_buffers, key=span)
         self._first = [span(t)[0] for t in self._written]
         self._reach = list(accumulate((span(t)[1] for t in self._written), max))
-        mats, self._spans = [], []
+        mats, self._at = [], []
         for p, m in zip(params, self.momentum_buffers):
-            ps, ms = _slices(p), _slices(m)
-            self._spans.append((len(mats), len(ps)))
-            mats += [MuonMatrix(p.shape[-2], p.shape[-1], None, 0, b, a, _ld(p)) for a, b in zip(ps, ms)]
+            self._at.append(len(mats))
+            mats += [MuonMatrix(p.shape[-2], p.shape[-1], None, 0, b, a, _ld(p)) for a, b in zip(_slices(p), _slices(m))]
         self._mats = (MuonMatrix * len(mats))(*mats)
-        with on_device(self.device):
-            self._ws_bytes = lib.check(lib.mctsq_muon_workspace_bytes(self._mats, len(mats)))
-            self._ws = _aligned(self._ws_bytes, self.device)
-            self._ws_stream = stream_ptr(self.device)
+        self._placed = self._places()
+
+    def _follow(self):
+        """Parameters or momentum that have moved since the last step are written where they are now."""
+        now = self._places()
+        if now == self._placed:
+            return
+        if [p[1] for p in now] != [p[1] for p in self._placed]:
+            raise ValueError("params / momentum_buffers: their shapes have changed, make a new DeviceMuon")
+        self._check_params(self.params, self.device)
+        self._lay_out()
 
     def step(self, grads, lr=None):
         """One update from `grads` (a sequence in the order of the parameters)."""
+        self._follow()
         if len(grads) != len(self.params):
             raise ValueError(f"grads: expected {len(self.params)} tensors, got {len(grads)}")
         dt = grads[0].dtype
         if dt not in _DTYPE:
             raise ValueError(f"grads: expected fp32 or bf16, got {dt}")
-        for i, (g, p, (at, _)) in enumerate(zip(grads, self.params, self._spans)):
+        for i, (g, p, at) in enumerate(zip(grads, self.params, self._at)):
             if g.shape != p.shape or g.dtype != dt or g.device != self.device or not _is_matrix(g):
                 raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {dt} on {self.device} with contiguous rows, got "
                                  f"{tuple(g.shape)} {g.dtype} with strides {g.stride()} on {g.device}")
