@@ -3,6 +3,7 @@ ranges would refuse interleaved views, or pass views that cross each other's row
 from __future__ import annotations
 
 import numpy as np
+import torch
 
 
 def span(t):
@@ -72,3 +73,9 @@ def share_memory(a, b):
     at, to = _starts(a, da), _starts(b, db)
     k = np.searchsorted(to, at + ra) - 1                     # the last run of b that starts before this one of a ends
     return bool(((k >= 0) & (to[np.maximum(k, 0)] + rb > at)).any())
+
+
+def wrote(*tensors):
+    """Tell autograd, and whoever prepared something from these tensors, that a kernel changed them: torch's own in-place
+    operations count a version, a kernel's writes do not.  Tensors of inference mode carry none; a graph's replay counts nothing."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])

@@ -12,7 +12,7 @@ from itertools import accumulate
 import torch
 
 from ._lib import MctsqError, MuonMatrix, lib, on_device, ptr, stream_ptr
-from ._memory import overlaps_itself, share_memory, span
+from ._memory import overlaps_itself, share_memory, span, wrote
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 _ADJUST = {"none": 0, "spectral": 1, "rms": 2}
@@ -66,7 +66,8 @@ def orthogonalize(x, eps=1e-7, out=None):
     if not _is_matrix(x):
         raise ValueError(f"x: expected [rows, cols] or [count, rows, cols] with contiguous rows, got {tuple(x.shape)} "
                          f"with strides {x.stride()}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not _is_matrix(out) or overlaps_itself(out):
         raise ValueError(f"out: expected {tuple(x.shape)} {x.dtype} on {x.device} with contiguous rows that do not overlap")
@@ -81,6 +82,8 @@ def orthogonalize(x, eps=1e-7, out=None):
         need = lib.check(lib.mctsq_orthogonalize_workspace_bytes(mats, len(src), dt))
         ws = _aligned(need, x.device)
         lib.check(lib.mctsq_orthogonalize(mats, len(src), dt, eps, ptr(ws), need, stream_ptr(x.device)))
+    if given:
+        wrote(out)
     return out
 
 
@@ -189,6 +192,7 @@ class DeviceMuon:
             lib.check(lib.mctsq_muon_step(self._mats, len(self._mats), _DTYPE[dt], self.lr if lr is None else float(lr),
                                           self.momentum, int(self.nesterov), self.weight_decay, self.eps,
                                           _ADJUST[self.adjust], ptr(self._ws), self._ws_bytes, stream_ptr(self.device)))
+        wrote(*self.params, *self.momentum_buffers)
 
     def state_dict(self):
         return {"momentum_buffers": [m.clone() for m in self.momentum_buffers]}

@@ -19,7 +19,7 @@ import functools
 import torch
 
 from ._lib import MctsqError, lib, on_device, ptr, stream_ptr
-from ._memory import share_memory
+from ._memory import share_memory, wrote
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -125,6 +125,8 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, weight=Non
                                         actions.element_size(), ptr(old_logp), ptr(ref_logp), ptr(advantages), adv_div,
                                         ptr(weight), clip_low, clip_high, kl_coef, loss_scale, ptr(loss), ptr(logp),
                                         ptr(kl), ptr(d), dso, dsi, ptr(ws), need, stream_ptr(dev)))
+    if out is not None:
+        wrote(out)
     return dict(loss=loss, logp=logp, kl=kl, dlogits=d)
 
 
@@ -164,4 +166,6 @@ def preference_loss(logits, actions, ref_logp, weight=None, beta=0.1, label_smoo
                                             actions.element_size(), ptr(ref_logp), ptr(weight), ptr(pair_weight), beta,
                                             label_smoothing, loss_scale, ptr(loss), ptr(seq), ptr(margin), ptr(d), dso,
                                             dsi, ptr(ws), need, stream_ptr(dev)))
+    if out is not None:
+        wrote(out)
     return dict(loss=loss, seq_logp=seq, margin=margin, dlogits=d)
