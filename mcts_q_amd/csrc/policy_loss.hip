@@ -785,6 +785,12 @@ static int fill_grad(RowArgs& a, void* d_dlogits, int dtype, int64_t so, int64_t
     return 0;
 }
 
+// at most 2^58 rows: 20 bytes of workspace each and the sequences' own stay within 64 bits
+static int check_pairs(int64_t pairs, int64_t tokens) {
+    MCTSQ_CHECK(pairs >= 0 && tokens >= 0 && pairs <= ((int64_t)1 << 30) && tokens <= ((int64_t)1 << 31)
+                && 2 * pairs * tokens <= ((int64_t)1 << 58), "pairs / tokens out of range");
+    return 0;
+}
 static int64_t pref_ws(int64_t seqs, int64_t T, int64_t* off) {
     const int64_t rows = seqs * T;
     int64_t o = 0;
@@ -849,8 +855,7 @@ extern "C" int mctsq_policy_loss(const void* d_logits, int dtype, int64_t rows, 
 }
 
 extern "C" int64_t mctsq_preference_loss_workspace_bytes(int64_t pairs, int64_t tokens) {
-    MCTSQ_CHECK(pairs >= 0 && tokens >= 0, "negative size");
-    MCTSQ_CHECK(pairs <= ((int64_t)1 << 30) && tokens <= ((int64_t)1 << 31), "pairs / tokens out of range");
+    if (int rc = check_pairs(pairs, tokens)) return rc;
     int64_t off[6];
     return pref_ws(2 * pairs, tokens, off);
 }
@@ -861,8 +866,7 @@ extern "C" int mctsq_preference_loss(const void* d_logits, int dtype, int64_t pa
                                      double beta, double label_smoothing, double loss_scale, float* d_loss,
                                      float* d_seq_logp, float* d_margin, void* d_dlogits, int64_t dstride_outer,
                                      int64_t dstride_inner, void* d_ws, int64_t ws_bytes, void* stream) {
-    MCTSQ_CHECK(pairs >= 0 && tokens >= 0 && pairs <= ((int64_t)1 << 30) && tokens <= ((int64_t)1 << 31),
-                "pairs / tokens out of range");              // their product fits 64 bits
+    if (int rc = check_pairs(pairs, tokens)) return rc;
     const int64_t rows = 2 * pairs * tokens;
     RowArgs a;
     if (int rc = fill_rows(a, d_logits, dtype, rows, tokens > 0 ? tokens : 1, stride_outer, stride_inner, vocab, d_act, act_bytes, d_weight)) return rc;
