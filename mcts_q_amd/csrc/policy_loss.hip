@@ -331,7 +331,9 @@ __device__ __forceinline__ double exp_f64(double x) {
 __device__ __forceinline__ double expm1_f64(double x) {
     int k;
     const double p = exp_parts(x, k);
-    return x == x ? ldexp(p, k) + (ldexp(1.0, k) - 1.0) : x;
+    // from 2^60 on the 1 is below half a step; two parts of unlike signs would meet as infinities further up
+    const double v = k > 60 ? ldexp(1.0 + p, k) : ldexp(p, k) + (ldexp(1.0, k) - 1.0);
+    return x == x ? v : x;
 }
 
 // The row's log-probability and, in the policy mode, its loss and coefficient; writes the per-row outputs.
@@ -354,9 +356,11 @@ __device__ __forceinline__ double row_result(const RowArgs& a, int64_t row, floa
         if (un != un) loss = c = un;
         if (a.ref_logp) {
             const double d = (double)a.ref_logp[row] - logp, e = expm1_f64(d);
-            k = e - d;
-            loss += a.kl_coef * k;
-            c -= a.kl_coef * e;
+            k = e == INFINITY ? e : e - d;                               // d may be infinite
+            if (a.kl_coef != 0.0) {                                      // else k is only reported
+                loss += a.kl_coef * k;
+                c -= a.kl_coef * e;
+            }
         }
         a.kl[row] = (float)k;
         const double sw = a.scale * (double)w;
@@ -380,6 +384,9 @@ __device__ __forceinline__ void row_const(const RowArgs& a, int64_t row, float v
     if (MODE == MODE_LOGP && a.logp64) a.logp64[row] = (double)v;
 }
 
+// the action's own element, c - c p; of an infinite coefficient the formula's c (1 - p)
+__device__ __forceinline__ float at_action(float g, float coef) { return fabsf(coef) < INFINITY ? g + coef : coef; }
+
 // vector v of the gradient: g holds -c p, the action's own element gets its c
 template <typename T>
 __device__ __forceinline__ void put_grad(const RowView<T>& rv, char* out, bool aligned, int64_t v, float* g, int64_t a, float coef) {
@@ -387,7 +394,7 @@ __device__ __forceinline__ void put_grad(const RowView<T>& rv, char* out, bool a
     const int64_t ja = a + rv.mis - v * VE;             // the action's place in this vector, if it is here
     if (ja >= 0 && ja < VE)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) if (j == ja) g[j] += coef;
+        for (int j = 0; j < VE; ++j) if (j == ja) g[j] = at_action(g[j], coef);
     rv.store(out, aligned, v, g);
 }
 
@@ -596,7 +603,7 @@ __global__ __launch_bounds__(NT) void row_lane_kernel(RowArgs a) {
             for (int k = 0; k < EPL; ++k) {
                 const int64_t e = g + k * G;
                 if (e < a.V) {
-                    const float v = scale * (MODE == MODE_GRAD ? exp_diff(x[k], m) : x[k]) + (e == act ? coef : 0.0f);
+                    const float g0 = scale * (MODE == MODE_GRAD ? exp_diff(x[k], m) : x[k]), v = e == act ? at_action(g0, coef) : g0;
                     Elem<T>::store(out, e, live ? v : (bad ? NAN : 0.0f));
                 }
             }

@@ -1,0 +1,63 @@
+"""GPU: the policy losses where an exponential leaves the range of 64 bits.
+
+A ratio or a KL term of more than e^709 is infinite in 64 bits: the formula's limit is +inf, never NaN (which stands for an
+action that does not exist).  Elements of such a row's gradient are c (one_hot - p) with c = -inf: -inf at the action,
++inf where p > 0, and NaN only where an infinity meets p = 0."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _rows(V, dtype, n=9):
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = (torch.randn(n, V, generator=g, device="cuda") * 2).to(dtype)
+    a = torch.randint(0, V, (n,), generator=g, device="cuda")
+    return z, a, torch.log_softmax(z.double(), -1).gather(1, a[:, None])[:, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("V", [5, 30, 200, 700, 9001])
+def test_a_reference_far_above_the_policy(V, dtype):
+    """d = ref - logp: e^d - d - 1 grows without a bound; past 64 bits it is +inf whatever the fraction of d / log 2 is."""
+    from mcts_q_amd.policyloss import policy_loss
+    z, a, lp = _rows(V, dtype)
+    d = torch.tensor([0.5, 80.0, 200.0, 709.0, 720.0, 900.0, 1100.0, 5000.0, 1e30], device="cuda", dtype=torch.float64)
+    ref = (lp + d).float()
+    d = ref.double() - lp
+    adv = torch.ones(9, device="cuda")
+    k = d.exp() - d - 1
+    r = policy_loss(z, a, None, adv, ref_logp=ref, kl_coef=0.1)
+    assert not r["kl"].isnan().any()
+    small = torch.tensor([True, True] + [False] * 7, device="cuda")
+    assert (r["kl"][~small] == math.inf).all()                       # past fp32 from d = 89 on
+    # d itself is off by the log-probability's error, at most 250 u: a relative error of k of that size
+    assert ((r["kl"][small].double() - k[small]).abs() <= (250 * U + U) * 1.01 * (k + d + 1)[small]).all()
+    assert float(r["loss"]) == math.inf
+    far = d > 712
+    at = r["dlogits"].gather(1, a[:, None])[:, 0]
+    assert (at[far] == -math.inf).all()
+    assert not (r["dlogits"][far] < 0).scatter(1, a[far][:, None], False).any()
+    # the KL term only looked at: it takes no part in the loss
+    r = policy_loss(z, a, None, adv, ref_logp=ref, kl_coef=0.0)
+    assert float(r["loss"]) == -9.0 and torch.isfinite(r["dlogits"]).all() and (r["kl"][~small] == math.inf).all()
+    plain = policy_loss(z, a, None, adv)
+    assert torch.equal(plain["dlogits"], r["dlogits"])
+
+
+@pytest.mark.parametrize("V", [5, 700])
+def test_a_live_action_of_probability_zero(V):
+    """logit -inf at the action: logp = -inf, ratio 0, and the KL term +inf under a reference that is finite."""
+    from mcts_q_amd.policyloss import policy_loss
+    z, a, lp = _rows(V, torch.float32)
+    z[2, a[2]] = -math.inf
+    old = lp.float()
+    adv = torch.ones(9, device="cuda")
+    r = policy_loss(z, a, old, adv)
+    assert float(r["logp"][2]) == -math.inf and not r["dlogits"][2].any() and math.isfinite(float(r["loss"]))
+    r = policy_loss(z, a, old, adv, ref_logp=old, kl_coef=0.1)
+    assert float(r["kl"][2]) == math.inf and float(r["loss"]) == math.inf and float(r["dlogits"][2, a[2]]) == -math.inf
+    assert torch.isfinite(r["dlogits"][[0, 1, 3, 4, 5, 6, 7, 8]]).all()
