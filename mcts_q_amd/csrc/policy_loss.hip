@@ -351,7 +351,8 @@ __device__ __forceinline__ double row_result(const RowArgs& a, int64_t row, floa
     if constexpr (MODE == MODE_POLICY) {
         const double A = (double)a.adv[a.adv_div == 1 ? row : a.adv_div == a.inner ? row_group(a, row) : row / a.adv_div];
         const double r = a.old_logp ? exp_f64(logp - (double)a.old_logp[row]) : (logp == logp ? 1.0 : logp);
-        const double un = r * A, cl = fmin(fmax(r, a.clip_lo), a.clip_hi) * A;
+        // 0 where A is 0 and r infinite (a behaviour policy that gave the action no probability)
+        const double un = A == 0.0 && r == r ? 0.0 : r * A, cl = A == 0.0 ? 0.0 : fmin(fmax(r, a.clip_lo), a.clip_hi) * A;
         double loss = -(un <= cl ? un : cl), c = un <= cl ? -un : 0.0, k = 0.0;
         if (un != un) loss = c = un;
         if (a.ref_logp) {

@@ -96,9 +96,9 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, weight=Non
     """loss = loss_scale * sum_i w_i (-min(r_i A_i, clip(r_i, 1 - clip_low, 1 + clip_high) A_i) + kl_coef k_i) with
     r = exp(logp - old_logp) and k = exp(ref_logp - logp) - (ref_logp - logp) - 1.
 
-    old_logp None: on-policy, r = 1.  ref_logp None: no KL term; kl_coef 0: k is only reported.  advantages: one per row, or `[B]` for `[B, T, V]`
-    logits (one per sequence).  `out`: where the gradient goes, with strides of its own; the logits themselves are
-    allowed.  Returns dict(loss [1], logp, kl (k per row), dlogits (None when grad is False))."""
+    old_logp None: on-policy, r = 1.  ref_logp None: no KL term; kl_coef 0: k is only reported.  advantages: one per row,
+    or `[B]` for `[B, T, V]` logits (one per sequence).  `out`: where the gradient goes, with strides of its own; the logits
+    themselves are allowed.  Returns dict(loss [1], logp, kl (k per row), dlogits (None when grad is False))."""
     n, inner, so, si, V, lead = _rows(logits, actions)
     dev = logits.device
     for name, t in (("old_logp", old_logp), ("ref_logp", ref_logp), ("weight", weight)):

@@ -61,3 +61,22 @@ def test_a_live_action_of_probability_zero(V):
     r = policy_loss(z, a, old, adv, ref_logp=old, kl_coef=0.1)
     assert float(r["kl"][2]) == math.inf and float(r["loss"]) == math.inf and float(r["dlogits"][2, a[2]]) == -math.inf
     assert torch.isfinite(r["dlogits"][[0, 1, 3, 4, 5, 6, 7, 8]]).all()
+
+
+@pytest.mark.parametrize("V", [5, 700])
+def test_an_infinite_ratio(V):
+    """A behaviour policy that gave the action (next to) no probability: r = +inf.  A positive advantage is clipped, a
+    negative one is an infinite loss, an advantage of 0 takes no part."""
+    from mcts_q_amd.policyloss import policy_loss
+    z, a, lp = _rows(V, torch.float32)
+    old = lp.float()
+    old[0], old[1], old[2] = -math.inf, -5000.0, -750.0
+    adv = torch.zeros(9, device="cuda")
+    r = policy_loss(z, a, old, adv)
+    assert float(r["loss"]) == 0.0 and not r["dlogits"].any()
+    adv[:3] = 2.0
+    r = policy_loss(z, a, old, adv, clip_high=0.25)
+    assert float(r["loss"]) == -7.5 and not r["dlogits"].any()       # 3 * 1.25 * 2, on the flat side
+    adv[0] = -2.0
+    r = policy_loss(z, a, old, adv)
+    assert float(r["loss"]) == math.inf
