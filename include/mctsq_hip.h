@@ -261,7 +261,7 @@ int mctsq_polyak(const float* d_params, float* d_target, int64_t n, double tau, 
  * reported only); exponentials past 64 bits are +inf, and an advantage of 0 takes no part whatever the ratio is.  d_adv: row i
  * uses d_adv[i / adv_div] (adv_div = 1: one per row; = inner: one per sequence).  Outputs: d_loss [1], d_logp [rows], d_kl
  * [rows] (k_i; 0 without a reference), d_dlogits or NULL: the gradient of the loss in the logits' type with its own strides;
- * it may be the logits themselves (same pointer and strides), else must not overlap them.  Where the unclipped product equals
+ * it may be the logits themselves (same pointer and strides), else must not overlap them or anything read.  Where the unclipped product equals
  * the clipped one the gradient is the unclipped one's.
  *
  * mctsq_preference_loss: 2 * pairs sequences of `tokens` rows, the preferred ones first; S_q = sum_t w_qt logp_qt,

@@ -63,7 +63,7 @@ def _vec(name, t, shape, device):
                          f"{t.device}")
 
 
-def _grad_out(logits, out):
+def _grad_out(logits, out, **read):
     if out is None:
         return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
@@ -72,6 +72,9 @@ def _grad_out(logits, out):
                          f"{tuple(out.shape)} {out.dtype} on {out.device}")
     if not (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()) and share_memory(logits, out):
         raise ValueError("out: must be the logits themselves or share no memory with them")
+    for name, t in read.items():                             # other rows still read them while this one's gradient is written
+        if t is not None and share_memory(t, out):
+            raise ValueError(f"out: must share no memory with {name}")
     return out
 
 
@@ -113,7 +116,8 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, weight=Non
         _vec("advantages", advantages, lead, dev)
     if not grad and out is not None:
         raise ValueError("out is given but grad is False")
-    d = _grad_out(logits, out) if grad else None
+    d = _grad_out(logits, out, actions=actions, old_logp=old_logp, advantages=advantages, ref_logp=ref_logp,
+                  weight=weight) if grad else None
     dso, dsi = _out_strides(d) if grad else (0, 0)
     with on_device(dev):
         need = _policy_ws(n)
@@ -154,7 +158,7 @@ def preference_loss(logits, actions, ref_logp, weight=None, beta=0.1, label_smoo
         raise ValueError("out is given but grad is False")
     if loss_scale is None:
         loss_scale = 1.0 / max(P, 1)
-    d = _grad_out(logits, out) if grad else None
+    d = _grad_out(logits, out, actions=actions, ref_logp=ref_logp, weight=weight, pair_weight=pair_weight) if grad else None
     dso, dsi = _out_strides(d) if grad else (0, 0)
     with on_device(dev):
         need = _preference_ws(P, T)

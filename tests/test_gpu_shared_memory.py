@@ -83,3 +83,27 @@ def test_a_gradient_beside_its_logits(dtype):
             with pytest.raises(ValueError, match="out"):
                 f(out=bad)
     assert torch.equal(z, keep)
+
+
+def test_a_gradient_over_what_other_rows_read():
+    """Weights, actions, old log-probabilities in the memory that the gradient is written to: refused by name."""
+    from mcts_q_amd.policyloss import policy_loss, preference_loss
+    z = _rand((4, 6, 50), 1)
+    out = torch.zeros(4, 6, 50, device="cuda")
+    a, f, s = torch.zeros(4, 6, dtype=torch.int64, device="cuda"), torch.zeros(4, 6, device="cuda"), torch.zeros(4, device="cuda")
+    inside = out.view(-1)[100:124].view(4, 6)
+    act = out.view(-1)[100:148].view(torch.int64).view(4, 6)
+    vec = out.view(-1)[7:11]
+    for name, call in (("old_logp", lambda: policy_loss(z, a, inside, f, out=out)),
+                       ("advantages", lambda: policy_loss(z, a, f, inside, out=out)),
+                       ("advantages", lambda: policy_loss(z, a, f, vec, out=out)),
+                       ("ref_logp", lambda: policy_loss(z, a, f, f, ref_logp=inside, out=out)),
+                       ("weight", lambda: policy_loss(z, a, f, f, weight=inside, out=out)),
+                       ("actions", lambda: policy_loss(z, act, f, f, out=out)),
+                       ("actions", lambda: preference_loss(z, act, s, out=out)),
+                       ("ref_logp", lambda: preference_loss(z, a, vec, out=out)),
+                       ("weight", lambda: preference_loss(z, a, s, weight=inside, out=out)),
+                       ("pair_weight", lambda: preference_loss(z, a, s, pair_weight=vec[:2], out=out))):
+        with pytest.raises(ValueError, match=name):
+            call()
+    assert not out.any()
