@@ -180,10 +180,12 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 
 // Sum of exp(f - ref) over N values, left in f: four at a time in fp32, those sums in fp64 -- or, ACC, each in fp64 together
 // with what the exponentials' arguments lost.  Two log-probabilities' difference, rows of 32000 to 81298, rms against 64 bits:
-// 2.9e-8, ACC 1.0e-8 (what is left is the exponential instruction's own).  ACC is for fp32 logits (4096 x 32000: 92 -> 97 us,
-// with the gradient 202 -> 198) and for at most a row per CU, where no number of rows averages the errors and the call around
-// the launch takes longer (48 x 32000 bf16: 5.8 -> 7.2 us on the device, the call 10 either way); many 16-bit rows would pay
-// 25 % (45 -> 56 us).
+// 2.9e-8, ACC 1.0e-8 (what is left is the exponential instruction's own).  Either is below what a log-probability beyond -1/2
+// loses when it is stored in fp32, so a row in a short and in a long call gives the same value or its neighbour; a preference
+// margin and a ratio see the 64-bit value.  ACC is for fp32 logits (4096 x 32000: 92 -> 97 us, with the gradient 202 -> 198) and
+// for at most a row per CU, where the call around the launch takes longer than the kernel (48 x 32000 bf16: 5.8 -> 7.2 us on the
+// device, the call 10 either way).  Many 16-bit rows would pay for it: log-probabilities of 6 x 1023 x 50257 bf16 84 -> 106 us,
+// policy loss of 3 x 333 x 50257 fp16 51 -> 64, preference loss of 4 pairs x 61 x 32000 bf16 25.5 -> 28.4.
 template <int N, bool ACC>
 __device__ __forceinline__ double sum_exp(float* f, float ref) {
     double s = 0.0, t = 0.0;
@@ -719,8 +721,9 @@ static int64_t launch_rows(const RowArgs& a, hipStream_t st) {
     if (a.V <= 256) MCTSQ_ROWS(256, 16, row_lane_kernel<T, 16, 16, 256, MODE>);
     // Measured (policy loss, 2 V bytes a bf16 row, 33 to 270 MB of logits; GB/s read + written): waves per row and vectors
     // per lane so that one row just fits keeps the most rows in flight -- V = 2040 RW 1 U 4 3900 (RW 2 2830), 8184 RW 2 U 8
-    // 4780 (RW 4 3500), 16000 RW 4 U 8 5050 (RW 8 U 4 4340), 65000 RW 16 U 8 4660 (streamed 3880); only 32000 is better
-    // streamed by 8 waves (4150 against 3900) as two held rows are all that fit a CU; fp32 rows hold half as many
+    // 4780 (RW 4 3500), 16000 RW 4 U 8 5050 (RW 8 U 4 4340), 65000 RW 16 U 8 4660 (streamed 3880).  Between, 16-bit rows are
+    // better streamed by 8 waves, as two held rows are all that fit a CU: calls of 67 MB of logits, streamed / held, 17000
+    // 2960 / 2580, 20000 3110 / 2810, 24000 3440 / 3180, 28000 3510 / 3260, 32000 3550 / 3400; fp32 rows hold half as many
     // values per vector and have no such gap (32000: held 5220, streamed 4560).  131072 streamed by 16 waves 3840.
     // vectors of a row: at its worst alignment, unless every row starts on a vector
     const int64_t es = sizeof(T), starts = (int64_t)((uintptr_t)a.z & 15) | ((a.z_si | (a.one_group ? 0 : a.z_so)) * es & 15);
