@@ -316,7 +316,7 @@ __device__ __forceinline__ double log_f64(double s) {
 // e^x = 2^k (1 + p), p = e^r - 1 by its series, |r| <= log(2) / 2
 __device__ __forceinline__ double exp_parts(double x, int& k) {
     const double lim = scalar_const(1100.0), c = fmin(fmax(x, -lim), lim), n = rint(c * scalar_const(1.4426950408889634));
-    // log 2 in two words
+    // log 2 as its first 32 bits after the point, which n times are exact, and the rest
     const double r = fma(-n, scalar_const(1.9082149292705877e-10), fma(-n, scalar_const(0.6931471803691238), c));
     constexpr double fact[13] = {1, 1, 2, 6, 24, 120, 720, 5040, 40320, 362880, 3628800, 39916800, 479001600};
     double p = scalar_const(1.0 / fact[12]);
@@ -651,12 +651,18 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
     double acc[8];                                                        // [pair of four][side]
 #pragma unroll
     for (int q = 0; q < 8; ++q) acc[q] = 0.0;
+    bool live[4];                                                         // padding pairs: nothing of theirs counts
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int64_t p = base + wave + 16 * q;
+        live[q] = p < a.P && !(a.pair_w && a.pair_w[p] == 0.0f);
+    }
     for (int64_t t = lane; t < a.T; t += 64) {                            // eight loads under way, each sum in order
         double v[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             const int64_t p = base + wave + 16 * (q >> 1), row = (p + (q & 1) * a.P) * a.T + t;
-            const bool in = p < a.P;
+            const bool in = live[q >> 1];
             const float w = in ? (a.w ? a.w[row] : 1.0f) : 0.0f;
             const double l = in ? a.logp64[row] : 0.0;
             v[q] = w != 0.0f ? (double)w * l : 0.0;

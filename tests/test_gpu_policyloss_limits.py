@@ -80,3 +80,25 @@ def test_an_infinite_ratio(V):
     adv[0] = -2.0
     r = policy_loss(z, a, old, adv)
     assert float(r["loss"]) == math.inf
+
+
+@pytest.mark.parametrize("V", [5, 700])
+def test_padding_pairs_with_weights_of_nothing(V):
+    """Row weights 1 / length of an empty sequence are 0 / 0: in a pair of weight 0 they are not looked at."""
+    from mcts_q_amd.policyloss import preference_loss
+    P, T = 70, 3
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = torch.randn(2 * P, T, V, generator=g, device="cuda")
+    a = torch.randint(0, V, (2 * P, T), generator=g, device="cuda")
+    ref = torch.zeros(2 * P, device="cuda")
+    w, u = torch.full((2 * P, T), 1 / 3, device="cuda"), torch.ones(P, device="cuda")
+    want = preference_loss(z, a, ref, weight=w, pair_weight=u)
+    for p in (1, 66):
+        w[p], w[P + p], u[p] = math.nan, math.inf, 0.0
+    r = preference_loss(z, a, ref, weight=w, pair_weight=u)
+    gone = torch.zeros(P, dtype=torch.bool, device="cuda")
+    gone[[1, 66]] = True
+    assert not r["seq_logp"][gone.repeat(2)].any() and not r["margin"][gone].any() and not r["dlogits"][gone.repeat(2)].any()
+    assert math.isfinite(float(r["loss"]))
+    assert torch.equal(r["seq_logp"][~gone.repeat(2)], want["seq_logp"][~gone.repeat(2)])
+    assert torch.equal(r["dlogits"][~gone.repeat(2)], want["dlogits"][~gone.repeat(2)])
