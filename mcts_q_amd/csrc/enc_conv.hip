@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void conv_enc_fwd_kernel(ConvFwdArgs args, 
         if (t > 0) pc.attend(L.pool, cur, t - 1, s.sv_score, row0, Bp);
         float v[4];
 #pragma unroll
-        for (int pp = 0; pp < 2; ++pp) {                         // packed pairs of rows: the step is bound by vector issue
+        for (int pp = 0; pp < 2; ++pp) {                         // pairs of rows
             const f32x2 sm = ((f32x2){acc0[2 * pp], acc0[2 * pp + 1]} + (f32x2){acc1[2 * pp], acc1[2 * pp + 1]}) +
                              (f32x2){acc2[2 * pp], acc2[2 * pp + 1]};
             const f32x2 y = sm * inv2 + b2j;

@@ -715,7 +715,7 @@ static int64_t launch_rows(const RowArgs& a, hipStream_t st) {
     } while (0)
     const int64_t bytes = a.V * (int64_t)sizeof(T);
     if (a.V <= 8) {
-        // a lane per row.  Up to 1024 rows (the agent's batch of 1024 over 5 actions) one workgroup takes them all and adds
+        // a lane per row.  Up to 1024 rows (a batch of 1024 over 5 actions) one workgroup takes them all and adds
         // its own loss up: one launch
         if (MODE == MODE_POLICY && a.rows <= 1024) {
             hipLaunchKernelGGL((row_lane_kernel<T, 1, 8, 1024, MODE>), dim3(1), dim3(1024), 0, st, a);

@@ -31,7 +31,7 @@ struct PoolCore {
         float4 ps;
 #pragma unroll
         for (int r = 0; r < 4; ++r) h[r] = v[r];
-        const f32x2 a01 = (f32x2){v[0], v[1]} * awj, a23 = (f32x2){v[2], v[3]} * awj;      // packed pairs of rows
+        const f32x2 a01 = (f32x2){v[0], v[1]} * awj, a23 = (f32x2){v[2], v[3]} * awj;      // pairs of rows
         ps.x = row16_sum(a01.x); ps.y = row16_sum(a01.y); ps.z = row16_sum(a23.x); ps.w = row16_sum(a23.y);
         // one lane per row group stores its four sums as 16 bytes; the others write theirs to a slot of their own:
         // no branch around the store (gru_core.hpp: GruWave::publish)
@@ -43,7 +43,7 @@ struct PoolCore {
         float4 sp[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) sp[w] = *reinterpret_cast<const float4*>(&L.spart[buf][w][4 * q]);
-        // the four waves' partial scores summed on packed pairs of rows
+        // the four waves' partial scores summed on pairs of rows
         const f32x2 s01 = (((f32x2){sp[0].x, sp[0].y} + (f32x2){sp[1].x, sp[1].y}) + ((f32x2){sp[2].x, sp[2].y} + (f32x2){sp[3].x, sp[3].y})) + ab;
         const f32x2 s23 = (((f32x2){sp[0].z, sp[0].w} + (f32x2){sp[1].z, sp[1].w}) + ((f32x2){sp[2].z, sp[2].w} + (f32x2){sp[3].z, sp[3].w})) + ab;
         const float scs[4] = {s01.x, s01.y, s23.x, s23.y};

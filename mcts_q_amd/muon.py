@@ -96,7 +96,8 @@ class DeviceMuon:
     f by `adjust`: "spectral" sqrt(max(1, rows / cols)), "rms" 0.2 sqrt(max(rows, cols)), "none" 1.  A parameter is
     [rows, cols] or a stack [count, rows, cols] of matrices, rows contiguous.  Gradients are fp32 or bf16, all of one type.
     They share no memory with the parameters or the state: `momentum_buffers` (fp32, contiguous, one per parameter).  The
-    workspace is kept, so steps of one instance belong on one stream at a time (two graphs captured from one instance must
+    workspace is kept (8 bytes an element and 16 per square of the smaller side, of the largest twenty neighbours in the list),
+    so steps of one instance belong on one stream at a time (two graphs captured from one instance must
     not run at once), and an instance has to live as long as the graphs captured from it.  Parameters that move between
     steps (`p.data = ...`) are followed; a captured graph keeps the addresses it was captured with."""
 
