@@ -349,12 +349,16 @@ class _AdamFacade:
                            "params": by_muon})
         return {"state": state, "param_groups": groups}
 
+    @staticmethod
+    def _muon_group(sd):
+        return next((g for g in sd["param_groups"] if g.get("optimizer") == "muon"), None)
+
     def check_state_dict(self, sd):
         """ValueError where the state is the other optimizer's.  A single group without the mark is Adam's, or Muon's
         momentum written as exp_avg with exp_avg_sq 0, told by its values: m^2 <= 53 v in Adam, so its m is below 1e-16
         where v rounded to 0."""
         muon = self.learner.optimizer == "muon"
-        marked = any(g.get("optimizer") == "muon" for g in sd["param_groups"])
+        marked = self._muon_group(sd)
         theirs = [sd["state"][i] for i in self._muon_indices() if i in sd["state"]]
         if not marked:
             momentum = [not s["exp_avg_sq"].any() and float(s["exp_avg"].abs().max()) > 1e-16 for s in theirs]
@@ -365,7 +369,7 @@ class _AdamFacade:
         if not muon and (marked or any(momentum)):
             raise ValueError("the optimizer state is Muon's, this model's optimizer is Adam: build it with optimizer='muon', "
                              "or load the networks alone")
-        if marked and sd["param_groups"][1]["params"] != self._muon_indices():
+        if marked and list(marked["params"]) != self._muon_indices():
             raise ValueError("the optimizer state's Muon matrices are not this network's")
 
     def load_state_dict(self, sd):
@@ -383,8 +387,8 @@ class _AdamFacade:
                 m[k].copy_(s["exp_avg"]); v[k].copy_(s["exp_avg_sq"])
         g = sd["param_groups"][0]
         self.lr = L.lr = float(g["lr"]); L.betas = tuple(g["betas"]); L.eps = float(g["eps"])
-        if len(sd["param_groups"]) > 1:
-            g = sd["param_groups"][1]
+        g = self._muon_group(sd)
+        if g:
             L.muon.lr, L.muon.momentum, L.muon.nesterov = float(g["lr"]), float(g["momentum"]), bool(g["nesterov"])
             L.muon.weight_decay, L.muon.eps, L.muon.adjust = float(g["weight_decay"]), float(g["eps"]), g["adjust"]
 

@@ -110,3 +110,17 @@ def test_before_the_first_step():
     one, two = _model("muon", steps=0), _model("muon", seed=8, steps=1)
     two.optimizer.load_state_dict(one.optimizer.state_dict())
     assert two.learner.step_count == 0 and not two.learner.exp_avg.any()
+
+
+def test_adam_state_in_several_groups():
+    """Only the mark makes a group Muon's: an Adam state of two groups is Adam's, its first group gives the settings."""
+    a, b = _model("adam"), _model("adam", seed=8)
+    sd = a.optimizer.state_dict()
+    n = len(sd["param_groups"][0]["params"])
+    sd["param_groups"] = [dict(sd["param_groups"][0], params=list(range(n // 2))),
+                          dict(sd["param_groups"][0], params=list(range(n // 2, n)), lr=0.5)]
+    b.optimizer.load_state_dict(sd)
+    assert torch.equal(a.learner.exp_avg, b.learner.exp_avg) and torch.equal(a.learner.exp_avg_sq, b.learner.exp_avg_sq)
+    assert b.learner.step_count == 3 and b.learner.lr == 1e-3
+    with pytest.raises(ValueError, match="Muon"):
+        _model("muon", seed=9, steps=1).optimizer.load_state_dict(sd)
